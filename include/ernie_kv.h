@@ -690,6 +690,150 @@ int ekv_import_fp8_ds_mla_pages(const uint8_t* src, int64_t src_page_stride /*by
                                 int64_t page_stride /*bytes*/, int64_t num_pages, const int32_t* dst_pages,
                                 void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Grouped-query layers: H query heads share kv_heads key / value heads (H a
+ * multiple of kv_heads) of dim channels (64, 128 or 256), as dense draft
+ * models beside the MLA layers have.  No counterpart in the reference, whose
+ * layers cache latent rows only.
+ *
+ *   page      64 tokens; e4m3fn codes with one power-of-two scale for the keys
+ *             and one for the values of each kv head:
+ *             K codes at (64 h + r) dim + c (head h, token r, channel c);
+ *             V codes at 64 dim kv_heads + (dim h + c) 64 + at(r),
+ *               at(r) = 16 ((r / 4) % 4) + 4 (r / 16) + r % 4;
+ *             then fp32 K scales [kv_heads], then fp32 V scales [kv_heads].
+ *             Pages are page_stride bytes apart (a multiple of 16, at least
+ *             ekv_gqa_page_bytes); the cache is 16-byte aligned.
+ *   scale     2^ceil(log2(max(amax, 1e-10) * (1/448))) of the head's rows; a
+ *             page that goes on keeps the larger of its own and the new rows'
+ *             scale, and its earlier codes are requantized where it grows.
+ *   summary   for each page the mean key of each head as dim int8 codes, then
+ *             fp32 scales [kv_heads] (2^ceil(log2(max(amax, 1e-10) * (1/127)))
+ *             of the mean's code values, times the K scale); records
+ *             summary_stride bytes apart (a multiple of 16, at least
+ *             ekv_gqa_summary_bytes).
+ *   page ids  block_table[seq][position / 64], bt_width entries a row; ids
+ *             outside [0, num_pages) and positions behind the row are skipped.
+ *   inputs    finite; strides in elements, channels contiguous.
+ * ------------------------------------------------------------------------- */
+
+/* Bytes of a page / of a page's summary, rounded up to 16 (0: dim or kv_heads
+ * not supported). */
+int64_t ekv_gqa_page_bytes(int32_t kv_heads, int32_t dim);
+int64_t ekv_gqa_summary_bytes(int32_t kv_heads, int32_t dim);
+
+/*
+ * RMS norm of every query and key head (x * rsqrt(mean x^2 + eps) * w, fp32;
+ * a null w leaves the norm out) and the rotation of `rope` channels from
+ * rope_offset on by row positions[t] of cos_sin [cos_sin_rows, rope] fp32
+ * (cos rope/2 | sin rope/2), on pairs (i, i + rope/2) or, interleaved, (2i,
+ * 2i + 1); rounded once to bf16.  q [T, heads, dim], k [T, kv_heads, dim] bf16,
+ * dim a multiple of 16 up to 512, rope a multiple of 16 (0: no rotation),
+ * rope_offset of 8; weights [dim] fp32 or bf16; outputs contiguous and 16-byte
+ * aligned.  Positions outside the table leave the row unrotated.
+ */
+int ekv_qk_norm_rope(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int32_t heads,
+                     const uint16_t* k, int64_t k_tok_stride, int64_t k_head_stride, int32_t kv_heads,
+                     int32_t num_tokens, int32_t dim, const void* q_w, const void* k_w, int32_t w_is_bf16,
+                     float eps, const float* cos_sin, int32_t cos_sin_rows, int32_t rope, int32_t rope_offset,
+                     int32_t interleaved, const int64_t* positions, uint16_t* q_out, uint16_t* k_out, void* stream);
+
+/*
+ * Cache write: k, v [T, kv_heads, dim] bf16 of sequences b (tokens qsl[b] ..
+ * qsl[b+1]-1, at most max_query_len, at consecutive positions from
+ * positions[qsl[b]] on; a negative first position skips the sequence) into
+ * their pages.  A row at position p rewrites its page's earlier rows only
+ * where the scale grows, and leaves the bytes behind the call's last row as
+ * they were.  summary (may be NULL) gets the record of every page written: the
+ * mean of its rows up to the call's last.  No two sequences may write the same
+ * page in one call.
+ */
+int ekv_gqa_append(const uint16_t* k, int64_t k_tok_stride, int64_t k_head_stride, const uint16_t* v,
+                   int64_t v_tok_stride, int64_t v_head_stride, int32_t num_tokens, int32_t kv_heads, int32_t dim,
+                   const int64_t* positions, const int32_t* qsl, int32_t num_seqs, int32_t max_query_len,
+                   const int32_t* block_table, int64_t bt_stride, int32_t bt_width, uint8_t* cache,
+                   int64_t page_stride /*bytes*/, int64_t num_pages, uint8_t* summary,
+                   int64_t summary_stride /*bytes*/, void* stream);
+
+/*
+ * ekv_qk_norm_rope of q and k (dim 64, 128 or 256) and ekv_gqa_append of the
+ * result, in one launch and with the same bytes: q_out [T, heads, dim], the
+ * prepared keys go to the cache only.
+ */
+int ekv_gqa_prologue(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int32_t heads,
+                     const uint16_t* k, int64_t k_tok_stride, int64_t k_head_stride, const uint16_t* v,
+                     int64_t v_tok_stride, int64_t v_head_stride, int32_t num_tokens, int32_t kv_heads, int32_t dim,
+                     const void* q_w, const void* k_w, int32_t w_is_bf16, float eps, const float* cos_sin,
+                     int32_t cos_sin_rows, int32_t rope, int32_t rope_offset, int32_t interleaved,
+                     const int64_t* positions, const int32_t* qsl, int32_t num_seqs, int32_t max_query_len,
+                     const int32_t* block_table, int64_t bt_stride, int32_t bt_width, uint8_t* cache,
+                     int64_t page_stride /*bytes*/, int64_t num_pages, uint8_t* summary,
+                     int64_t summary_stride /*bytes*/, uint16_t* q_out, void* stream);
+
+/* Workspace bytes of ekv_gqa_attention for the same sizes (0: none needed). */
+int64_t ekv_gqa_attention_workspace_size(int32_t num_tokens, int32_t num_seqs, int32_t max_query_len,
+                                         int32_t max_len, int32_t heads, int32_t kv_heads, int32_t dim,
+                                         int32_t window);
+
+/*
+ * Causal attention over the pages: row t of sequence b (qsl as above) sees the
+ * tokens j <= positions[t] and, with window > 0, j > positions[t] - window:
+ *   out [T, heads, dim] bf16 = sum_j e^{s_j} v_j / (sum_j e^{s_j} + e^{sink}),
+ *   s_j = scale q . k_j; lse [T, heads] fp32 = log sum_j e^{s_j} (may be NULL).
+ * sinks [heads] fp32 may be NULL.  A row that sees no token (a negative
+ * position) gets zeros and -inf; rows of no sequence are left as they were.
+ * max_query_len and max_len bound the rows and the tokens of a sequence.  What
+ * lies behind a sequence's last token is never used, whatever its bytes.
+ * workspace (16-byte aligned) holds the partial results of long sequences;
+ * calls that share one must not overlap.
+ */
+int ekv_gqa_attention(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int32_t num_tokens,
+                      int32_t heads, int32_t kv_heads, int32_t dim, const uint8_t* cache,
+                      int64_t page_stride /*bytes*/, int64_t num_pages, const int32_t* block_table,
+                      int64_t bt_stride, int32_t bt_width, const int64_t* positions, const int32_t* qsl,
+                      int32_t num_seqs, int32_t max_query_len, int32_t max_len, int32_t window, const float* sinks,
+                      float scale, uint16_t* out, int64_t out_tok_stride, int64_t out_head_stride, float* lse,
+                      int64_t lse_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The pages that each query token and kv head attends to: scores
+ * max_g (q_g . m_j) s_j over the heads g of the group, with q as int8 codes
+ * (2^ceil(log2(max(amax, 1e-10) * (1/127))) of the group, which the score leaves
+ * out) and m_j, s_j page j's summary; exact in fp32.  blocks [T, kv_heads,
+ * num_blocks] int32 gets the num_blocks best of the pages 0 .. positions[t] / 64
+ * of request req_ids[t] (lowest index first on ties) in ascending order, -1
+ * behind them; the first keep_first and the last keep_last pages come before all
+ * others.  Pages outside the cache are not taken; a request id outside
+ * [0, num_seqs) leaves the row as it was.  At most 64 heads a kv head and
+ * 2^21 tokens.
+ */
+int ekv_gqa_block_select(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int32_t num_tokens,
+                         int32_t heads, int32_t kv_heads, int32_t dim, const uint8_t* summary,
+                         int64_t summary_stride /*bytes*/, int64_t num_pages, const int32_t* block_table,
+                         int64_t bt_stride, int32_t bt_width, const int64_t* positions, const int32_t* req_ids,
+                         int32_t num_seqs, int32_t max_len, int32_t keep_first, int32_t keep_last, int32_t* blocks,
+                         int64_t blocks_tok_stride, int64_t blocks_head_stride, int32_t num_blocks, void* stream);
+
+/* Workspace bytes of ekv_gqa_block_attention for the same sizes. */
+int64_t ekv_gqa_block_attention_workspace_size(int32_t num_tokens, int32_t heads, int32_t kv_heads, int32_t dim,
+                                               int32_t num_blocks);
+
+/*
+ * ekv_gqa_attention over the listed pages alone: blocks [T, kv_heads,
+ * num_blocks] int32 as ekv_gqa_block_select writes them (negative entries and
+ * pages behind the row's position are skipped, an entry listed twice counts
+ * twice), tokens up to positions[t] of request req_ids[t]; a request id outside
+ * [0, num_seqs) leaves the row as it was.
+ */
+int ekv_gqa_block_attention(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int32_t num_tokens,
+                            int32_t heads, int32_t kv_heads, int32_t dim, const uint8_t* cache,
+                            int64_t page_stride /*bytes*/, int64_t num_pages, const int32_t* block_table,
+                            int64_t bt_stride, int32_t bt_width, const int64_t* positions, const int32_t* req_ids,
+                            int32_t num_seqs, const int32_t* blocks, int64_t blocks_tok_stride,
+                            int64_t blocks_head_stride, int32_t num_blocks, const float* sinks, float scale,
+                            uint16_t* out, int64_t out_tok_stride, int64_t out_head_stride, float* lse,
+                            int64_t lse_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,562 @@
+// Causal attention of grouped-query layers over 8-bit pages: every page of a
+// sequence (gqa_attention) or the pages a row selected (gqa_block_attention).
+//
+//   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sink)),  s_j = scale q . k_j
+//   lse = log sum_j exp(s_j)
+//
+// over the tokens j a row sees: j <= position and, with a window,
+// j > position - window.
+#include <algorithm>
+
+#include "ekv_gqa.h"
+
+namespace ekv {
+
+constexpr float kLog2e = 0x1.715476p+0f;
+constexpr float kLn2 = 0x1.62e430p-1f;
+constexpr float kNone = -1e30f;   // reference of a row that has seen no token
+constexpr float kSlack = 8.0f;    // log2 units over a row's reference that move it
+constexpr int kMaxSplits = 64;
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+struct GqaAttnArgs {
+  const uint16_t* q;
+  int64_t q_tok_stride, q_head_stride;
+  int32_t q_aligned, num_tokens, heads, kv_heads, group;
+  const uint8_t* cache;
+  int64_t page_stride, num_pages;
+  const int32_t* block_table;
+  int64_t bt_stride;
+  int32_t bt_width, num_seqs;
+  const int64_t* positions;
+  const int32_t* qsl;       // dense: [B + 1]
+  const int32_t* req_ids;   // selected blocks: [T]
+  const int32_t* ids;       // selected blocks: [T, kv_heads, n_ids] logical pages, -1 skipped
+  int64_t ids_tok_stride, ids_head_stride;
+  int32_t n_ids;
+  int32_t window;           // 0: none
+  float scale_log2;
+  const float* sinks;
+  uint16_t* out;
+  int64_t out_tok_stride, out_head_stride;
+  float* lse;
+  int64_t lse_stride;
+  // plan
+  int32_t tiles, units, splits, split_pages;
+  float* ws_o;              // [splits, T, heads, D]
+  float2* ws_ml;            // [splits, T, heads]: (reference in log2 units, sum)
+};
+
+// 8 e4m3fn codes times a power of two -> bf16.
+__device__ __forceinline__ bf16x8 fp8x8_to_bf16(uint32_t lo, uint32_t hi, float s) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
+  return __builtin_bit_cast(bf16x8, make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                                               __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)));
+}
+
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
+__device__ __forceinline__ bf16x8 load_q8(const uint16_t* p, bool aligned) {
+  if (aligned) return __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(p));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = p[2 * i] | static_cast<uint32_t>(p[2 * i + 1]) << 16;
+  return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+// Result of a row whose weights sum to l around the reference m: 4 channels.
+__device__ __forceinline__ void store_out4(const GqaAttnArgs& a, int64_t t, int hq, int c, f32x4 o, float m, float l) {
+  float den = l;
+  if (a.sinks) den += __builtin_amdgcn_exp2f(a.sinks[hq] * kLog2e - m);
+  const float inv = den > 0.0f ? 1.0f / den : (den == den ? 0.0f : den);
+  const uint32_t lo = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(o[0] * inv), static_cast<__bf16>(o[1] * inv)});
+  const uint32_t hi = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(o[2] * inv), static_cast<__bf16>(o[3] * inv)});
+  uint16_t* p = a.out + t * a.out_tok_stride + hq * a.out_head_stride + c;
+  *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+}
+
+__device__ __forceinline__ void store_lse(const GqaAttnArgs& a, int64_t t, int hq, float m, float l) {
+  if (a.lse) a.lse[t * a.lse_stride + hq] = l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows a kv head: one workgroup per (16 NT rows, kv head, range of pages).
+// Each of its 4 waves takes every fourth page of the range through registers,
+// with no LDS in the loop: K as the A operand (16 tokens x 32 channels) against
+// q leaves a lane the scores of one row and of the tokens whose V bytes it
+// loads, so the weights go straight into the product with V.
+// ---------------------------------------------------------------------------
+template <int D, int NT, bool LIST>
+__global__ void __launch_bounds__(256) gqa_decode_kernel(GqaAttnArgs a) {
+  constexpr int S = D / 64, DT = D / 16;
+  __shared__ float so[4][16][D + 4];
+  __shared__ float2 sml[4][16];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int unit = static_cast<int>(blockIdx.x) % a.units, split = static_cast<int>(blockIdx.x) / a.units;
+  const int h = unit % a.kv_heads, tile = unit / a.kv_heads % a.tiles, seq = unit / a.kv_heads / a.tiles;
+
+  // the rows: (token, head of the group), flattened
+  int t0, rows, b;
+  if (LIST) {
+    t0 = seq, rows = a.group, b = a.req_ids[seq];
+    if (b < 0 || b >= a.num_seqs) return;
+  } else {
+    b = seq, t0 = a.qsl[b];
+    rows = (min(a.qsl[b + 1], a.num_tokens) - t0) * a.group;
+    if (t0 < 0) return;
+  }
+  const int r0 = tile * 16 * NT;
+  if (r0 >= rows) return;
+  int pos[NT], lo[NT], pmax = -1, pmin = 0x7fffffff, pany = 0x7fffffff;
+  bf16x8 q[NT][S][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = r0 + 16 * nt + n;
+    const bool have = r < rows;
+    const int tok = have ? r / a.group : 0, hq = h * a.group + (have ? r - tok * a.group : 0);
+    pos[nt] = 0x7fffffff;  // no row: unmasked zeros, never stored
+    if (have) {
+      pos[nt] = static_cast<int>(min(max(a.positions[t0 + tok], -1ll), 0x3fffffffll));
+      pmax = max(pmax, pos[nt]);
+      pany = min(pany, pos[nt]);
+      if (pos[nt] >= 0) pmin = min(pmin, pos[nt]);
+    }
+    lo[nt] = a.window ? pos[nt] - a.window + 1 : 0;  // the row sees lo .. pos
+    const uint16_t* src = a.q + (t0 + tok) * a.q_tok_stride + hq * a.q_head_stride + 16 * g;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        q[nt][s][u] = bf16x8{};
+        if (have) q[nt][s][u] = load_q8(src + 64 * s + 8 * u, a.q_aligned);
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) {
+    pmax = max(pmax, __shfl_xor(pmax, m, 64));
+    pmin = min(pmin, __shfl_xor(pmin, m, 64));
+    pany = min(pany, __shfl_xor(pany, m, 64));
+  }
+  pmax = __builtin_amdgcn_readfirstlane(pmax);
+  pmin = __builtin_amdgcn_readfirstlane(pmin);
+  pany = __builtin_amdgcn_readfirstlane(pany);
+  const int low = a.window && pmax >= 0 ? max(pmin - a.window + 1, 0) : 0;  // first token any row sees
+
+  int pb, pe;
+  if (LIST) {
+    pb = split * a.split_pages, pe = split == a.splits - 1 ? a.n_ids : min(pb + a.split_pages, a.n_ids);
+  } else {
+    const int last = pmax < 0 ? 0 : min(pmax / kPageTokens + 1, a.bt_width);
+    pb = low / kPageTokens + split * a.split_pages;
+    pe = split == a.splits - 1 ? last : min(pb + a.split_pages, last);
+  }
+
+  f32x4 o[NT][DT] = {};
+  float m[NT], l[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) m[nt] = kNone, l[nt] = 0.0f;
+
+  const int64_t k_at = static_cast<int64_t>(h) * kPageTokens * D + n * D + 16 * g;
+  const int64_t v_at = static_cast<int64_t>(a.kv_heads + h) * kPageTokens * D + n * kPageTokens + 16 * g;
+  const int32_t* bt = a.block_table + b * a.bt_stride;
+
+  for (int p0 = pb + wave; p0 < pe; p0 += 256) {
+    // lane i: the wave's i-th page of the next 64, its place and its scales
+    const int e = p0 + 4 * lane;
+    int lp = -1, page = -1;
+    float ks = 0.0f, vs = 0.0f;
+    if (e < pe) lp = LIST ? a.ids[t0 * a.ids_tok_stride + h * a.ids_head_stride + e] : e;
+    if (lp >= 0 && lp < a.bt_width && lp * static_cast<int64_t>(kPageTokens) <= pmax) page = bt[lp];
+    if (page >= a.num_pages) page = -1;
+    if (page >= 0) {
+      const float* sc = reinterpret_cast<const float*>(a.cache + page * a.page_stride +
+                                                       2ll * a.kv_heads * kPageTokens * D) + h;
+      ks = sc[0], vs = sc[a.kv_heads];
+    }
+    uint64_t todo = __ballot(page >= 0);
+    if (!todo) continue;
+    uint4 kr[4][S], vr[DT];
+    int at = __builtin_ctzll(todo);
+    {
+      const uint8_t* pg = a.cache + static_cast<int64_t>(__builtin_amdgcn_readlane(page, at)) * a.page_stride;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) kr[j][s] = *reinterpret_cast<const uint4*>(pg + k_at + 16 * j * D + 64 * s);
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const uint4*>(pg + v_at + 16 * d * kPageTokens);
+    }
+    while (true) {
+      todo &= todo - 1;
+      const int next = todo ? __builtin_ctzll(todo) : -1;
+      const uint8_t* ng =
+          a.cache + static_cast<int64_t>(__builtin_amdgcn_readlane(page, next < 0 ? at : next)) * a.page_stride;
+      const int first = __builtin_amdgcn_readlane(lp, at) * kPageTokens;
+      const float kscale = lane_value(ks, at) * a.scale_log2, vscale = lane_value(vs, at);
+
+      f32x4 x[NT][4] = {};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const bf16x8 k0 = fp8x8_to_bf16(kr[j][s].x, kr[j][s].y, 1.0f), k1 = fp8x8_to_bf16(kr[j][s].z, kr[j][s].w, 1.0f);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            x[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[nt][s][0], x[nt][j], 0, 0, 0);
+            x[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[nt][s][1], x[nt][j], 0, 0, 0);
+          }
+        }
+      }
+      if (next >= 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int s = 0; s < S; ++s) kr[j][s] = *reinterpret_cast<const uint4*>(ng + k_at + 16 * j * D + 64 * s);
+        }
+      }
+
+      const bool whole = first + kPageTokens - 1 <= pany && (!a.window || first > pmax - a.window);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[nt][j] *= kscale;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int from = lo[nt] - first - 4 * g, to = pos[nt] - first - 4 * g;  // seen: from <= 16 j + i <= to
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int at = 16 * j + i;
+              x[nt][j][i] = (at >= from) & (at <= to) ? x[nt][j][i] : -__builtin_inff();
+            }
+          }
+        }
+      }
+      float most = kNone;  // of x over its reference
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float top = x[nt][0][0];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, x[nt][j][i]);
+        }
+        most = fmaxf(most, top - m[nt]);
+      }
+      if (__any(most > kSlack)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float top = m[nt];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, x[nt][j][i]);
+          }
+          top = fmaxf(top, __shfl_xor(top, 16, 64));
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float f = __builtin_amdgcn_exp2f(m[nt] - top);
+          m[nt] = top;
+          l[nt] *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[nt][d] *= f;
+        }
+      }
+      bf16x8 w[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float y = __builtin_amdgcn_exp2f(x[nt][j][i] - m[nt]);
+            l[nt] += y;
+            w[nt][j >> 1][4 * (j & 1) + i] = static_cast<__bf16>(y);
+          }
+        }
+      }
+      if (!whole) {  // bytes behind the last token, or before the first, may be anything
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          uint32_t keep = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tok = first + 16 * t + 4 * g + i;
+            if (tok <= pmax && tok >= low) keep |= 0xffu << (8 * i);
+          }
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            if (t == 0) vr[d].x &= keep;
+            else if (t == 1) vr[d].y &= keep;
+            else if (t == 2) vr[d].z &= keep;
+            else vr[d].w &= keep;
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const bf16x8 v0 = fp8x8_to_bf16(vr[d].x, vr[d].y, vscale), v1 = fp8x8_to_bf16(vr[d].z, vr[d].w, vscale);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, w[nt][0], o[nt][d], 0, 0, 0);
+          o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, w[nt][1], o[nt][d], 0, 0, 0);
+        }
+      }
+      if (next < 0) break;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vr[d] = *reinterpret_cast<const uint4*>(ng + v_at + 16 * d * kPageTokens);
+      at = next;
+    }
+  }
+
+  // the four waves' parts of each row
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    l[nt] += __shfl_xor(l[nt], 16, 64);
+    l[nt] += __shfl_xor(l[nt], 32, 64);
+    if (nt) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&so[wave][n][16 * d + 4 * g]) = o[nt][d];
+    if (g == 0) sml[wave][n] = make_float2(m[nt], l[nt]);
+    __syncthreads();
+    const int row = tid >> 4, r = r0 + 16 * nt + row;
+    if (r >= rows) continue;
+    const int64_t t = t0 + r / a.group;
+    const int hq = h * a.group + r % a.group;
+    float top = kNone, sum = 0.0f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, sml[w][row].x);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(sml[w][row].x - top);
+      sum += f[w] * sml[w][row].y;
+    }
+#pragma unroll
+    for (int c = 4 * (tid & 15); c < D; c += 64) {
+      f32x4 y = {};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) y += f[w] * *reinterpret_cast<const f32x4*>(&so[w][row][c]);
+      if (a.splits == 1) {
+        store_out4(a, t, hq, c, y, top, sum);
+      } else {
+        *reinterpret_cast<f32x4*>(a.ws_o + ((static_cast<int64_t>(split) * a.num_tokens + t) * a.heads + hq) * D + c) = y;
+      }
+    }
+    if ((tid & 15) == 0) {
+      if (a.splits == 1) store_lse(a, t, hq, top, sum);
+      else a.ws_ml[(static_cast<int64_t>(split) * a.num_tokens + t) * a.heads + hq] = make_float2(top, sum);
+    }
+  }
+}
+
+// Joins the splits: one wave per (token, head), lane s the s-th split's weight.
+template <int D, bool LIST>
+__global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t t = row / a.heads;
+  const int hq = static_cast<int>(row - t * a.heads);
+  if (t >= a.num_tokens) return;
+  if (LIST) {
+    if (a.req_ids[t] < 0 || a.req_ids[t] >= a.num_seqs) return;
+  } else {
+    if (t < a.qsl[0] || t >= a.qsl[a.num_seqs]) return;
+  }
+  const int64_t step = static_cast<int64_t>(a.num_tokens) * a.heads;
+  float2 ml = make_float2(kNone, 0.0f);
+  if (lane < a.splits) ml = a.ws_ml[lane * step + row];
+  float top = ml.x;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  const float f = __builtin_amdgcn_exp2f(ml.x - top);
+  float sum = f * ml.y;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m, 64);
+  uint64_t todo = __ballot(ml.y != 0.0f);
+  const int c = 4 * lane;
+  f32x4 y = {};
+  while (todo) {
+    const int s = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    const float fs = lane_value(f, s);
+    if (c < D) y += fs * *reinterpret_cast<const f32x4*>(a.ws_o + (s * step + row) * D + c);
+  }
+  if (c < D) store_out4(a, t, hq, c, y, top, sum);
+  if (lane == 0) store_lse(a, t, hq, top, sum);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+struct GqaPlan {
+  int row_tiles;  // 16-row tiles a workgroup takes
+  int tiles, splits, split_pages;
+  int64_t units;
+};
+
+// seqs: sequences (dense) or tokens (selected blocks); rows: query rows a kv head has in each.
+static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int kv_heads, int dim, int64_t pages) {
+  GqaPlan p{};
+  const int most = dim == 256 ? 1 : dim == 128 ? 2 : 4;
+  p.row_tiles = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+  p.tiles = static_cast<int>((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
+  p.units = seqs * kv_heads * p.tiles;
+  pages = std::max<int64_t>(pages, 1);
+  int64_t splits = std::min<int64_t>({(1024 + p.units - 1) / std::max<int64_t>(p.units, 1), (pages + 3) / 4, kMaxSplits});
+  splits = std::max<int64_t>(splits, 1);
+  p.split_pages = static_cast<int>((pages + splits - 1) / splits);
+  p.splits = static_cast<int>((pages + p.split_pages - 1) / p.split_pages);
+  return p;
+}
+
+static int64_t dense_pages(int64_t max_len, int64_t max_query_len, int64_t window) {
+  int64_t pages = (max_len + kPageTokens - 1) / kPageTokens;
+  if (window) pages = std::min(pages, (window + max_query_len - 2) / kPageTokens + 2);
+  return pages;
+}
+
+static int64_t plan_bytes(const GqaPlan& p, int64_t num_tokens, int64_t heads, int64_t dim) {
+  return p.splits == 1 ? 0 : p.splits * num_tokens * heads * (dim + 2) * 4;
+}
+
+template <int D, bool LIST>
+static int launch_decode(const GqaAttnArgs& a, int row_tiles, hipStream_t s) {
+  const int64_t blocks = static_cast<int64_t>(a.units) * a.splits;
+  EKV_CHECK(blocks < (int64_t{1} << 31), "too many rows for one call");
+  const dim3 grid(static_cast<uint32_t>(blocks));
+  if (row_tiles == 1) gqa_decode_kernel<D, 1, LIST><<<grid, 256, 0, s>>>(a);
+  if constexpr (D <= 128) {
+    if (row_tiles == 2) gqa_decode_kernel<D, 2, LIST><<<grid, 256, 0, s>>>(a);
+  }
+  if constexpr (D == 64) {
+    if (row_tiles == 4) gqa_decode_kernel<D, 4, LIST><<<grid, 256, 0, s>>>(a);
+  }
+  int rc = ekv_launch_status();
+  if (rc || a.splits == 1) return rc;
+  const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.heads;
+  gqa_combine_kernel<D, LIST><<<dim3(static_cast<uint32_t>((rows + 3) / 4)), 256, 0, s>>>(a);
+  return ekv_launch_status();
+}
+
+template <bool LIST>
+static int launch_attn(GqaAttnArgs& a, const GqaPlan& p, int dim, void* workspace, int64_t workspace_bytes,
+                       void* stream) {
+  EKV_CHECK(p.units < (int64_t{1} << 31), "too many rows for one call");
+  const int64_t need = plan_bytes(p, a.num_tokens, a.heads, dim);
+  if (need > workspace_bytes || (need && !workspace)) {
+    set_error("workspace too small");
+    return kWorkspaceTooSmall;
+  }
+  EKV_CHECK(!need || aligned16(workspace), "workspace must be 16-byte aligned");
+  a.tiles = p.tiles, a.units = static_cast<int32_t>(p.units), a.splits = p.splits, a.split_pages = p.split_pages;
+  a.ws_o = static_cast<float*>(workspace);
+  a.ws_ml = reinterpret_cast<float2*>(a.ws_o + static_cast<int64_t>(p.splits) * a.num_tokens * a.heads * dim);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dim == 64) return launch_decode<64, LIST>(a, p.row_tiles, s);
+  if (dim == 128) return launch_decode<128, LIST>(a, p.row_tiles, s);
+  return launch_decode<256, LIST>(a, p.row_tiles, s);
+}
+
+static int attn_args(GqaAttnArgs& a, const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride,
+                     int32_t num_tokens, int32_t heads, int32_t kv_heads, int32_t dim, const uint8_t* cache,
+                     int64_t page_stride, int64_t num_pages, const int32_t* block_table, int64_t bt_stride,
+                     int32_t bt_width, const int64_t* positions, int32_t num_seqs, const float* sinks, float scale,
+                     uint16_t* out, int64_t out_tok_stride, int64_t out_head_stride, float* lse, int64_t lse_stride) {
+  EKV_CHECK(gqa_dim(dim), "dim must be 64, 128 or 256");
+  EKV_CHECK(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "heads must be a multiple of kv_heads");
+  EKV_CHECK(num_tokens >= 0 && num_seqs >= 0 && num_pages >= 0 && bt_width >= 0, "negative sizes");
+  a = GqaAttnArgs{};
+  if (!num_tokens || !num_seqs) return kOk;
+  EKV_CHECK(q && cache && block_table && positions && out, "null pointer");
+  EKV_CHECK(page_stride >= gqa_page_bytes(kv_heads, dim) && page_stride % 16 == 0 && aligned16(cache),
+            "page_stride must be a multiple of 16 of at least kv_heads * (128 * dim + 8) bytes");
+  EKV_CHECK(aligned8(out) && out_tok_stride % 4 == 0 && out_head_stride % 4 == 0,
+            "out rows must start at 8-byte addresses");
+  EKV_CHECK(num_pages < (int64_t{1} << 31) && bt_width <= (1 << 24), "too many pages");
+  a.q = q, a.q_tok_stride = q_tok_stride, a.q_head_stride = q_head_stride;
+  a.q_aligned = aligned16(q) && q_tok_stride % 8 == 0 && q_head_stride % 8 == 0;
+  a.num_tokens = num_tokens, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
+  a.cache = cache, a.page_stride = page_stride, a.num_pages = num_pages;
+  a.block_table = block_table, a.bt_stride = bt_stride, a.bt_width = bt_width, a.num_seqs = num_seqs;
+  a.positions = positions, a.sinks = sinks, a.scale_log2 = scale * kLog2e;
+  a.out = out, a.out_tok_stride = out_tok_stride, a.out_head_stride = out_head_stride;
+  a.lse = lse, a.lse_stride = lse_stride;
+  return kOk;
+}
+
+}  // namespace ekv
+
+using namespace ekv;
+
+extern "C" int64_t ekv_gqa_attention_workspace_size(int32_t num_tokens, int32_t num_seqs, int32_t max_query_len,
+                                                    int32_t max_len, int32_t heads, int32_t kv_heads, int32_t dim,
+                                                    int32_t window) {
+  if (num_tokens <= 0 || num_seqs <= 0 || max_query_len <= 0 || kv_heads <= 0 || heads < kv_heads || !gqa_dim(dim) ||
+      window < 0)
+    return 0;
+  const int64_t rows = std::min(max_query_len, num_tokens);
+  return plan_bytes(gqa_plan(num_seqs, rows * (heads / kv_heads), kv_heads, dim,
+                             dense_pages(std::max(max_len, 0), rows, window)),
+                    num_tokens, heads, dim);
+}
+
+extern "C" int ekv_gqa_attention(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int32_t num_tokens,
+                                 int32_t heads, int32_t kv_heads, int32_t dim, const uint8_t* cache,
+                                 int64_t page_stride, int64_t num_pages, const int32_t* block_table,
+                                 int64_t bt_stride, int32_t bt_width, const int64_t* positions, const int32_t* qsl,
+                                 int32_t num_seqs, int32_t max_query_len, int32_t max_len, int32_t window,
+                                 const float* sinks, float scale, uint16_t* out, int64_t out_tok_stride,
+                                 int64_t out_head_stride, float* lse, int64_t lse_stride, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  GqaAttnArgs a;
+  const int rc = attn_args(a, q, q_tok_stride, q_head_stride, num_tokens, heads, kv_heads, dim, cache, page_stride,
+                           num_pages, block_table, bt_stride, bt_width, positions, num_seqs, sinks, scale, out,
+                           out_tok_stride, out_head_stride, lse, lse_stride);
+  if (rc) return rc;
+  EKV_CHECK(max_query_len >= 0 && max_len >= 0 && window >= 0, "negative sizes");
+  if (!a.num_tokens || !max_query_len) return kOk;
+  EKV_CHECK(qsl, "null pointer");
+  a.qsl = qsl, a.window = window;
+  const int64_t rows = std::min(max_query_len, num_tokens);
+  return launch_attn<false>(a, gqa_plan(num_seqs, rows * a.group, kv_heads, dim, dense_pages(max_len, rows, window)),
+                            dim, workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t ekv_gqa_block_attention_workspace_size(int32_t num_tokens, int32_t heads, int32_t kv_heads,
+                                                          int32_t dim, int32_t num_blocks) {
+  if (num_tokens <= 0 || kv_heads <= 0 || heads < kv_heads || !gqa_dim(dim)) return 0;
+  return plan_bytes(gqa_plan(num_tokens, heads / kv_heads, kv_heads, dim, num_blocks), num_tokens, heads, dim);
+}
+
+extern "C" int ekv_gqa_block_attention(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride,
+                                       int32_t num_tokens, int32_t heads, int32_t kv_heads, int32_t dim,
+                                       const uint8_t* cache, int64_t page_stride, int64_t num_pages,
+                                       const int32_t* block_table, int64_t bt_stride, int32_t bt_width,
+                                       const int64_t* positions, const int32_t* req_ids, int32_t num_seqs,
+                                       const int32_t* blocks, int64_t blocks_tok_stride, int64_t blocks_head_stride,
+                                       int32_t num_blocks, const float* sinks, float scale, uint16_t* out,
+                                       int64_t out_tok_stride, int64_t out_head_stride, float* lse,
+                                       int64_t lse_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+  GqaAttnArgs a;
+  const int rc = attn_args(a, q, q_tok_stride, q_head_stride, num_tokens, heads, kv_heads, dim, cache, page_stride,
+                           num_pages, block_table, bt_stride, bt_width, positions, num_seqs, sinks, scale, out,
+                           out_tok_stride, out_head_stride, lse, lse_stride);
+  if (rc) return rc;
+  EKV_CHECK(num_blocks >= 0 && num_blocks <= (1 << 24), "negative sizes");
+  if (!a.num_tokens) return kOk;
+  EKV_CHECK(req_ids && (blocks || !num_blocks), "null pointer");
+  a.req_ids = req_ids, a.ids = blocks, a.ids_tok_stride = blocks_tok_stride, a.ids_head_stride = blocks_head_stride;
+  a.n_ids = num_blocks;
+  return launch_attn<true>(a, gqa_plan(num_tokens, a.group, kv_heads, dim, num_blocks), dim, workspace,
+                           workspace_bytes, stream);
+}

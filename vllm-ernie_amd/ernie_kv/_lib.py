@@ -114,6 +114,38 @@ SIGNATURES: dict[str, tuple] = {
     "ekv_indexer_filter_dots_fp4": (I32, [P, P, P, P, I32, P, P]),
     "ekv_export_fp8_ds_mla_pages": (I32, [P, I64, I64, P, I32, P, I64, I64, P, P]),
     "ekv_import_fp8_ds_mla_pages": (I32, [P, I64, I64, P, I32, P, I64, I64, P, P]),
+    "ekv_gqa_page_bytes": (I64, [I32, I32]),
+    "ekv_gqa_summary_bytes": (I64, [I32, I32]),
+    "ekv_qk_norm_rope": (
+        I32,
+        [P, I64, I64, I32, P, I64, I64, I32, I32, I32, P, P, I32, F32, P, I32, I32, I32, I32, P, P, P, P],
+    ),
+    "ekv_gqa_append": (
+        I32,
+        [P, I64, I64, P, I64, I64, I32, I32, I32, P, P, I32, I32, P, I64, I32, P, I64, I64, P, I64, P],
+    ),
+    "ekv_gqa_prologue": (
+        I32,
+        [P, I64, I64, I32, P, I64, I64, P, I64, I64, I32, I32, I32, P, P, I32, F32, P, I32, I32, I32, I32,
+         P, P, I32, I32, P, I64, I32, P, I64, I64, P, I64, P, P],
+    ),
+    "ekv_gqa_attention_workspace_size": (I64, [I32, I32, I32, I32, I32, I32, I32, I32]),
+    "ekv_gqa_attention": (
+        I32,
+        [P, I64, I64, I32, I32, I32, I32, P, I64, I64, P, I64, I32, P, P, I32, I32, I32, I32, P, F32, P,
+         I64, I64, P, I64, P, I64, P],
+    ),
+    "ekv_gqa_block_select": (
+        I32,
+        [P, I64, I64, I32, I32, I32, I32, P, I64, I64, P, I64, I32, P, P, I32, I32, I32, I32, P, I64, I64,
+         I32, P],
+    ),
+    "ekv_gqa_block_attention_workspace_size": (I64, [I32, I32, I32, I32, I32]),
+    "ekv_gqa_block_attention": (
+        I32,
+        [P, I64, I64, I32, I32, I32, I32, P, I64, I64, P, I64, I32, P, P, I32, P, I64, I64, I32, P, F32, P,
+         I64, I64, P, I64, P, I64, P],
+    ),
 }
 
 _lib = None

@@ -51,6 +51,9 @@ SOURCES = {
     "ekv_quant.hip": EXACT,
     "ekv_mxfp4.hip": EXACT,
     "ekv_pages.hip": EXACT,
+    "ekv_gqa_write.hip": EXACT,
+    "ekv_gqa_attn.hip": [],
+    "ekv_gqa_select.hip": EXACT,
 }
 
 

@@ -1079,3 +1079,241 @@ def vha_inv_rope_fp8_quant(o: torch.Tensor, mix: torch.Tensor, positions: torch.
                   mix.data_ptr(), positions.data_ptr(), cos_sin_cache.data_ptr(), cos_sin_cache.stride(0),
                   int(n_groups), int(nope_dim), int(rope_dim), out.data_ptr(), scale.data_ptr(), aligned, _stream())
     return out.transpose(0, 1), scale.permute(2, 0, 1)[:T]
+
+
+# --------------------------------------------------------------------------- grouped-query layers
+# Query heads share kv heads over 8-bit pages with a scale for each (page, kv
+# head) (layout: include/ernie_kv.h).  These wrappers take tensors of any one
+# device and run on that device's current stream.
+def _gqa_device(first: torch.Tensor, *rest: torch.Tensor | None) -> torch.device:
+    dev = first.device
+    _check_dev(first, *rest)
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return dev
+
+
+def _gqa_call(dev: torch.device, name: str, *args) -> None:
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, stream)
+
+
+def _st(t: torch.Tensor, d: int) -> int:
+    """Stride of dim ``d``; of one entry or none, which no address depends on, the packed one."""
+    return t.stride(d) if t.shape[d] > 1 else math.prod(t.shape[d + 1:])
+
+
+def _heads3(t: torch.Tensor, what: str) -> tuple[int, int, int]:
+    _bits16(t)
+    _need(t.dim() == 3 and (t.shape[2] <= 1 or t.stride(2) == 1), f"{what} [T, heads, D] with unit channel stride")
+    return t.shape
+
+
+def _pages2(t: torch.Tensor, what: str) -> torch.Tensor:
+    _need(t.dtype == torch.uint8 and t.dim() == 2 and t.stride(1) == 1, f"{what} uint8 [pages, bytes]")
+    return t
+
+
+def _table(t: torch.Tensor) -> torch.Tensor:
+    _need(t.dtype == torch.int32 and t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), "block_table int32 [B, P]")
+    return t
+
+
+def _vector(t: torch.Tensor, dtype, n: int, what: str) -> None:
+    _need(t.dtype == dtype and t.dim() == 1 and t.numel() >= n and (t.numel() <= 1 or t.stride(0) == 1),
+          f"{what} {dtype} [{n}] contiguous")
+
+
+def gqa_page_bytes(kv_heads: int, dim: int) -> int:
+    """Bytes of a 64-token page of ``kv_heads`` heads of ``dim`` channels."""
+    return int(_lib.load().ekv_gqa_page_bytes(int(kv_heads), int(dim)))
+
+
+def gqa_summary_bytes(kv_heads: int, dim: int) -> int:
+    """Bytes of a page's summary record (its heads' mean keys)."""
+    return int(_lib.load().ekv_gqa_summary_bytes(int(kv_heads), int(dim)))
+
+
+def _norm_args(w1, w2, dim: int, cos_sin, rope_offset: int, interleaved: bool) -> tuple:
+    for w in (w1, w2):
+        if w is not None:
+            _need(w.shape == (dim,) and w.is_contiguous() and w.dtype in (torch.float32, torch.bfloat16),
+                  "norm weights fp32 or bf16 [D]")
+    _need(w1 is None or w2 is None or w1.dtype == w2.dtype, "both norm weights of one type")
+    w = w1 if w1 is not None else w2
+    rows = rope = 0
+    if cos_sin is not None:
+        _need(cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous(), "cos_sin fp32 [N, rope]")
+        rows, rope = cos_sin.shape
+    return (_ptr(w1), _ptr(w2), int(w is not None and w.dtype == torch.bfloat16)), (
+        _ptr(cos_sin), rows, rope, int(rope_offset), int(interleaved))
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_w: torch.Tensor | None, k_w: torch.Tensor | None, eps: float,
+                 cos_sin: torch.Tensor | None, positions: torch.Tensor, interleaved: bool = False,
+                 rope_offset: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of each head of ``q [T, H, D]`` and ``k [T, H_kv, D]`` (weights
+    ``[D]``, None: no norm) and the rotation of ``cos_sin.shape[1]`` channels
+    from ``rope_offset`` on by row ``positions[t]`` of ``cos_sin`` (cos | sin),
+    on pairs half the slice apart or, ``interleaved``, neighbours; fp32,
+    rounded once.  Returns new contiguous ``(q, k)``."""
+    dev = _gqa_device(q, k, q_w, k_w, cos_sin, positions)
+    T, H, D = _heads3(q, "q")
+    _need(_heads3(k, "k")[::2] == (T, D), "k must be [T, H_kv, D] like q")
+    _vector(positions, torch.int64, T, "positions")
+    weights, rope = _norm_args(q_w, k_w, D, cos_sin, rope_offset, interleaved)
+    q_out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+    k_out = torch.empty((T, k.shape[1], D), dtype=k.dtype, device=dev)
+    _gqa_call(dev, "ekv_qk_norm_rope", q.data_ptr(), _st(q, 0), _st(q, 1), H, k.data_ptr(), _st(k, 0), _st(k, 1),
+              k.shape[1], T, D, *weights, float(eps), *rope, positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr())
+    return q_out, k_out
+
+
+def _append_args(k, v, positions, qsl, max_query_len, block_table, cache, summary) -> tuple:
+    T, KV, D = _heads3(k, "k")
+    _need(_heads3(v, "v") == (T, KV, D), "v must be [T, H_kv, D] like k")
+    _vector(positions, torch.int64, T, "positions")
+    _vector(qsl, torch.int32, 1, "qsl")
+    B = qsl.numel() - 1
+    _need(_table(block_table).shape[0] >= B, "block_table needs a row for each sequence")
+    _pages2(cache, "cache")
+    if summary is not None:
+        _need(_pages2(summary, "summary").shape[0] >= cache.shape[0], "summary needs a record for each page")
+    return ((k.data_ptr(), _st(k, 0), _st(k, 1), v.data_ptr(), _st(v, 0), _st(v, 1), T, KV, D),
+            (positions.data_ptr(), qsl.data_ptr(), B, int(max_query_len), block_table.data_ptr(), _st(block_table, 0),
+             block_table.shape[1], cache.data_ptr(), _st(cache, 0), cache.shape[0], _ptr(summary),
+             0 if summary is None else _st(summary, 0)))
+
+
+def gqa_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, qsl: torch.Tensor, max_query_len: int,
+               block_table: torch.Tensor, cache: torch.Tensor, summary: torch.Tensor | None = None) -> None:
+    """Keys and values ``[T, H_kv, D]`` of the sequences ``qsl`` (each at
+    consecutive positions from its first on) into their pages of ``cache``, and
+    the written pages' mean keys into ``summary``."""
+    dev = _gqa_device(k, v, positions, qsl, block_table, cache, summary)
+    head, tail = _append_args(k, v, positions, qsl, max_query_len, block_table, cache, summary)
+    _gqa_call(dev, "ekv_gqa_append", *head, *tail)
+
+
+def gqa_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_w: torch.Tensor | None,
+                 k_w: torch.Tensor | None, eps: float, cos_sin: torch.Tensor | None, positions: torch.Tensor,
+                 qsl: torch.Tensor, max_query_len: int, block_table: torch.Tensor, cache: torch.Tensor,
+                 summary: torch.Tensor | None = None, interleaved: bool = False,
+                 rope_offset: int = 0) -> torch.Tensor:
+    """``qk_norm_rope`` of q and k and ``gqa_append`` of the prepared keys and
+    ``v`` in one launch, same bytes; returns the prepared ``q``."""
+    dev = _gqa_device(q, k, v, q_w, k_w, cos_sin, positions, qsl, block_table, cache, summary)
+    T, H, D = _heads3(q, "q")
+    _need(k.dim() == 3 and k.shape[0] == T and k.shape[2] == D, "k must be [T, H_kv, D] like q")
+    head, tail = _append_args(k, v, positions, qsl, max_query_len, block_table, cache, summary)
+    weights, rope = _norm_args(q_w, k_w, D, cos_sin, rope_offset, interleaved)
+    q_out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+    _gqa_call(dev, "ekv_gqa_prologue", q.data_ptr(), _st(q, 0), _st(q, 1), H, *head, *weights, float(eps), *rope, *tail,
+              q_out.data_ptr())
+    return q_out
+
+
+def _gqa_attn_args(q, cache, kv_heads, block_table, positions, out, lse, sinks) -> tuple:
+    T, H, D = _heads3(q, "q")
+    _need(kv_heads > 0 and H % kv_heads == 0, "heads must be a multiple of kv_heads")
+    _pages2(cache, "cache")
+    _table(block_table)
+    _vector(positions, torch.int64, T, "positions")
+    _need(out.dtype == torch.bfloat16 and out.shape == (T, H, D) and out.stride(2) == 1, "out bf16 [T, H, D]")
+    if lse is not None:
+        _need(lse.dtype == torch.float32 and lse.shape == (T, H) and (H <= 1 or lse.stride(1) == 1), "lse fp32 [T, H]")
+    if sinks is not None:
+        _vector(sinks, torch.float32, H, "sinks")
+    return ((q.data_ptr(), _st(q, 0), _st(q, 1), T, H, int(kv_heads), D, cache.data_ptr(), _st(cache, 0),
+             cache.shape[0], block_table.data_ptr(), _st(block_table, 0), block_table.shape[1], positions.data_ptr()),
+            (out.data_ptr(), _st(out, 0), _st(out, 1), _ptr(lse), 0 if lse is None else _st(lse, 0)))
+
+
+def _gqa_workspace(workspace, need: int, dev) -> tuple:
+    if workspace is None:
+        if not need:
+            return None, (None, 0)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    _need(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.numel() >= need,
+          f"workspace too small: {workspace.numel()} < {need} bytes")
+    return workspace, (workspace.data_ptr(), workspace.numel())
+
+
+def gqa_attention_workspace(num_tokens: int, num_seqs: int, max_query_len: int, max_len: int, heads: int,
+                            kv_heads: int, dim: int, device, window: int = 0) -> torch.Tensor:
+    """Workspace of ``gqa_attention`` for calls of exactly these sizes."""
+    n = _lib.load().ekv_gqa_attention_workspace_size(num_tokens, num_seqs, max_query_len, max_len, heads, kv_heads, dim,
+                                                     window)
+    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=device)
+
+
+def gqa_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, block_table: torch.Tensor,
+                  positions: torch.Tensor, qsl: torch.Tensor, max_query_len: int, max_len: int, scale: float,
+                  out: torch.Tensor, lse: torch.Tensor | None = None, sinks: torch.Tensor | None = None,
+                  window: int = 0, workspace: torch.Tensor | None = None) -> None:
+    """Causal attention of ``q [T, H, D]`` over the pages of ``cache``: row t of
+    sequence b (``qsl``) sees the tokens up to ``positions[t]``, the last
+    ``window`` of them where it is not 0; ``sinks`` enter the denominator only.
+    Rows that see nothing get zeros and -inf, rows of no sequence stay."""
+    dev = _gqa_device(q, cache, block_table, positions, qsl, out, lse, sinks, workspace)
+    head, tail = _gqa_attn_args(q, cache, kv_heads, block_table, positions, out, lse, sinks)
+    _vector(qsl, torch.int32, 1, "qsl")
+    B, T, H, D = qsl.numel() - 1, *q.shape
+    _need(block_table.shape[0] >= B, "block_table needs a row for each sequence")
+    need = _lib.load().ekv_gqa_attention_workspace_size(T, B, int(max_query_len), int(max_len), H, int(kv_heads), D,
+                                                        int(window))
+    workspace, ws = _gqa_workspace(workspace, need, dev)
+    _gqa_call(dev, "ekv_gqa_attention", *head, qsl.data_ptr(), B, int(max_query_len), int(max_len), int(window),
+              _ptr(sinks), float(scale), *tail, *ws)
+
+
+def gqa_block_select(q: torch.Tensor, summary: torch.Tensor, kv_heads: int, block_table: torch.Tensor,
+                     positions: torch.Tensor, req_ids: torch.Tensor, max_len: int, blocks: torch.Tensor,
+                     keep_first: int = 1, keep_last: int = 2) -> None:
+    """``blocks [T, H_kv, n]`` int32: for each row and kv head the n pages with
+    the largest score against their mean keys, ascending, -1 behind them; the
+    first ``keep_first`` and the last ``keep_last`` pages come before others."""
+    dev = _gqa_device(q, summary, block_table, positions, req_ids, blocks)
+    T, H, D = _heads3(q, "q")
+    _need(kv_heads > 0 and H % kv_heads == 0, "heads must be a multiple of kv_heads")
+    _pages2(summary, "summary")
+    _table(block_table)
+    _vector(positions, torch.int64, T, "positions")
+    _vector(req_ids, torch.int32, T, "req_ids")
+    _need(blocks.dtype == torch.int32 and blocks.dim() == 3 and blocks.shape[:2] == (T, kv_heads)
+          and (blocks.shape[2] <= 1 or blocks.stride(2) == 1), "blocks int32 [T, H_kv, n]")
+    _gqa_call(dev, "ekv_gqa_block_select", q.data_ptr(), _st(q, 0), _st(q, 1), T, H, int(kv_heads), D,
+              summary.data_ptr(), _st(summary, 0), summary.shape[0], block_table.data_ptr(), _st(block_table, 0),
+              block_table.shape[1], positions.data_ptr(), req_ids.data_ptr(), block_table.shape[0], int(max_len),
+              int(keep_first), int(keep_last), blocks.data_ptr(), _st(blocks, 0), _st(blocks, 1), blocks.shape[2])
+
+
+def gqa_block_attention_workspace(num_tokens: int, heads: int, kv_heads: int, dim: int, num_blocks: int,
+                                  device) -> torch.Tensor:
+    """Workspace of ``gqa_block_attention`` for calls of exactly these sizes."""
+    n = _lib.load().ekv_gqa_block_attention_workspace_size(num_tokens, heads, kv_heads, dim, num_blocks)
+    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=device)
+
+
+def gqa_block_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, block_table: torch.Tensor,
+                        positions: torch.Tensor, req_ids: torch.Tensor, blocks: torch.Tensor, scale: float,
+                        out: torch.Tensor, lse: torch.Tensor | None = None, sinks: torch.Tensor | None = None,
+                        workspace: torch.Tensor | None = None) -> None:
+    """``gqa_attention`` over the pages that ``blocks [T, H_kv, n]`` lists for
+    each row and kv head (``gqa_block_select``; negative entries skipped)."""
+    dev = _gqa_device(q, cache, block_table, positions, req_ids, blocks, out, lse, sinks, workspace)
+    head, tail = _gqa_attn_args(q, cache, kv_heads, block_table, positions, out, lse, sinks)
+    T, H, D = q.shape
+    _vector(req_ids, torch.int32, T, "req_ids")
+    _need(blocks.dtype == torch.int32 and blocks.dim() == 3 and blocks.shape[:2] == (T, kv_heads)
+          and (blocks.shape[2] <= 1 or blocks.stride(2) == 1), "blocks int32 [T, H_kv, n]")
+    n = blocks.shape[2]
+    need = _lib.load().ekv_gqa_block_attention_workspace_size(T, H, int(kv_heads), D, n)
+    workspace, ws = _gqa_workspace(workspace, need, dev)
+    _gqa_call(dev, "ekv_gqa_block_attention", *head, req_ids.data_ptr(), block_table.shape[0], blocks.data_ptr(),
+              _st(blocks, 0), _st(blocks, 1), n, _ptr(sinks), float(scale), *tail, *ws)
