@@ -8,6 +8,7 @@ Caches are ``uint8`` tensors ``[num_pages, page_stride_bytes]``.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -1084,74 +1085,114 @@ def vha_inv_rope_fp8_quant(o: torch.Tensor, mix: torch.Tensor, positions: torch.
 # --------------------------------------------------------------------------- grouped-query layers
 # Query heads share kv heads over 8-bit pages with a scale for each (page, kv
 # head) (layout: include/ernie_kv.h).  These wrappers take tensors of any one
-# device and run on that device's current stream.
-def _gqa_device(first: torch.Tensor, *rest: torch.Tensor | None) -> torch.device:
-    dev = first.device
-    _check_dev(first, *rest)
-    for t in rest:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
+# device and run on that device's current stream.  A decode step calls them
+# for kernels of a few microseconds: each reads a tensor's shape and strides
+# once, and formats no message that it does not raise.
+def _refuse(msg: str) -> None:
+    raise ValueError(msg)
+
+
+def _gqa_device(*ts: torch.Tensor | None) -> int:
+    dev = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            _check_dev(*ts)
+            _refuse("tensors on different devices")
+    if dev < 0:
+        _check_dev(*ts)
     return dev
 
 
-def _gqa_call(dev: torch.device, name: str, *args) -> None:
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if dev.index == torch.cuda.current_device():
+def _gqa_call(dev: int, name: str, *args) -> None:
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch.cuda.current_device():
         _lib.call(name, *args, stream)
     else:
         with torch.cuda.device(dev):
             _lib.call(name, *args, stream)
 
 
-def _st(t: torch.Tensor, d: int) -> int:
-    """Stride of dim ``d``; of one entry or none, which no address depends on, the packed one."""
-    return t.stride(d) if t.shape[d] > 1 else math.prod(t.shape[d + 1:])
+def _heads3(t: torch.Tensor, what: str) -> tuple:
+    """(T, heads, D, token stride, head stride) of bf16 rows; the stride of a
+    dim of one entry, which no address depends on, is the packed one."""
+    if t.dtype is not torch.bfloat16:
+        _refuse(f"{what}: expected bfloat16, got {t.dtype}")
+    if t.dim() != 3:
+        _refuse(f"{what} [T, heads, D]")
+    T, H, D = t.shape
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and D > 1:
+        _refuse(f"{what} [T, heads, D] with unit channel stride")
+    return T, H, D, s0 if T > 1 else H * D, s1 if H > 1 else D
 
 
-def _heads3(t: torch.Tensor, what: str) -> tuple[int, int, int]:
-    _bits16(t)
-    _need(t.dim() == 3 and (t.shape[2] <= 1 or t.stride(2) == 1), f"{what} [T, heads, D] with unit channel stride")
-    return t.shape
+def _bytes2(t: torch.Tensor, what: str) -> tuple:
+    """(address, row stride, rows) of uint8 [rows, bytes]."""
+    if t.dtype is not torch.uint8 or t.dim() != 2 or t.stride(1) != 1:
+        _refuse(f"{what} uint8 [pages, bytes] with unit byte stride")
+    n, w = t.shape
+    return t.data_ptr(), t.stride(0) if n > 1 else w, n
 
 
-def _pages2(t: torch.Tensor, what: str) -> torch.Tensor:
-    _need(t.dtype == torch.uint8 and t.dim() == 2 and t.stride(1) == 1, f"{what} uint8 [pages, bytes]")
-    return t
+def _table(t: torch.Tensor, rows: int) -> tuple:
+    """(address, row stride, width) of a block table with at least ``rows`` rows."""
+    if t.dtype is not torch.int32 or t.dim() != 2:
+        _refuse("block_table int32 [B, P]")
+    b, p = t.shape
+    s0, s1 = t.stride()
+    if b < rows or (s1 != 1 and p > 1):
+        _refuse("block_table int32 [B, P] with a row for each sequence and unit stride in it")
+    return t.data_ptr(), s0 if b > 1 else p, p
 
 
-def _table(t: torch.Tensor) -> torch.Tensor:
-    _need(t.dtype == torch.int32 and t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), "block_table int32 [B, P]")
-    return t
+def _vector(t: torch.Tensor, dtype, n: int, what: str) -> int:
+    """Address of a contiguous vector of at least n entries."""
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
+        _refuse(f"{what} {dtype} [{n}] contiguous")
+    return t.data_ptr()
 
 
-def _vector(t: torch.Tensor, dtype, n: int, what: str) -> None:
-    _need(t.dtype == dtype and t.dim() == 1 and t.numel() >= n and (t.numel() <= 1 or t.stride(0) == 1),
-          f"{what} {dtype} [{n}] contiguous")
-
-
+@functools.lru_cache(maxsize=None)
 def gqa_page_bytes(kv_heads: int, dim: int) -> int:
     """Bytes of a 64-token page of ``kv_heads`` heads of ``dim`` channels."""
     return int(_lib.load().ekv_gqa_page_bytes(int(kv_heads), int(dim)))
 
 
+@functools.lru_cache(maxsize=None)
 def gqa_summary_bytes(kv_heads: int, dim: int) -> int:
     """Bytes of a page's summary record (its heads' mean keys)."""
     return int(_lib.load().ekv_gqa_summary_bytes(int(kv_heads), int(dim)))
 
 
-def _norm_args(w1, w2, dim: int, cos_sin, rope_offset: int, interleaved: bool) -> tuple:
-    for w in (w1, w2):
-        if w is not None:
-            _need(w.shape == (dim,) and w.is_contiguous() and w.dtype in (torch.float32, torch.bfloat16),
-                  "norm weights fp32 or bf16 [D]")
-    _need(w1 is None or w2 is None or w1.dtype == w2.dtype, "both norm weights of one type")
-    w = w1 if w1 is not None else w2
-    rows = rope = 0
+@functools.lru_cache(maxsize=4096)
+def _attention_bytes(*sizes: int) -> int:
+    return int(_lib.load().ekv_gqa_attention_workspace_size(*sizes))
+
+
+@functools.lru_cache(maxsize=4096)
+def _block_attention_bytes(*sizes: int) -> int:
+    return int(_lib.load().ekv_gqa_block_attention_workspace_size(*sizes))
+
+
+def _weight(w: torch.Tensor | None, dim: int) -> int | None:
+    if w is None:
+        return None
+    if w.dtype not in (torch.float32, torch.bfloat16) or w.dim() != 1 or w.shape[0] != dim or not w.is_contiguous():
+        _refuse("norm weights fp32 or bf16 [D] contiguous")
+    return w.data_ptr()
+
+
+def _norm_args(w1, w2, dim: int, eps: float, cos_sin, rope_offset: int, interleaved: bool) -> tuple:
+    if w1 is not None and w2 is not None and w1.dtype is not w2.dtype:
+        _refuse("both norm weights of one type")
+    w = w2 if w1 is None else w1
+    p, rows, rope = None, 0, 0
     if cos_sin is not None:
-        _need(cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous(), "cos_sin fp32 [N, rope]")
-        rows, rope = cos_sin.shape
-    return (_ptr(w1), _ptr(w2), int(w is not None and w.dtype == torch.bfloat16)), (
-        _ptr(cos_sin), rows, rope, int(rope_offset), int(interleaved))
+        if cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+            _refuse("cos_sin fp32 [N, rope] contiguous")
+        p, (rows, rope) = cos_sin.data_ptr(), cos_sin.shape
+    return (_weight(w1, dim), _weight(w2, dim), int(w is not None and w.dtype is torch.bfloat16), eps, p, rows, rope,
+            rope_offset, int(interleaved))
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_w: torch.Tensor | None, k_w: torch.Tensor | None, eps: float,
@@ -1163,31 +1204,33 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_w: torch.Tensor | None, k_w
     on pairs half the slice apart or, ``interleaved``, neighbours; fp32,
     rounded once.  Returns new contiguous ``(q, k)``."""
     dev = _gqa_device(q, k, q_w, k_w, cos_sin, positions)
-    T, H, D = _heads3(q, "q")
-    _need(_heads3(k, "k")[::2] == (T, D), "k must be [T, H_kv, D] like q")
-    _vector(positions, torch.int64, T, "positions")
-    weights, rope = _norm_args(q_w, k_w, D, cos_sin, rope_offset, interleaved)
-    q_out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    k_out = torch.empty((T, k.shape[1], D), dtype=k.dtype, device=dev)
-    _gqa_call(dev, "ekv_qk_norm_rope", q.data_ptr(), _st(q, 0), _st(q, 1), H, k.data_ptr(), _st(k, 0), _st(k, 1),
-              k.shape[1], T, D, *weights, float(eps), *rope, positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr())
+    T, H, D, q0, q1 = _heads3(q, "q")
+    Tk, KV, Dk, k0, k1 = _heads3(k, "k")
+    if T != Tk or D != Dk:
+        _refuse("k must be [T, H_kv, D] like q")
+    pos = _vector(positions, torch.int64, T, "positions")
+    norm = _norm_args(q_w, k_w, D, eps, cos_sin, rope_offset, interleaved)
+    q_out, k_out = q.new_empty((T, H, D)), k.new_empty((T, KV, D))
+    _gqa_call(dev, "ekv_qk_norm_rope", q.data_ptr(), q0, q1, H, k.data_ptr(), k0, k1, KV, T, D, *norm, pos,
+              q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
 def _append_args(k, v, positions, qsl, max_query_len, block_table, cache, summary) -> tuple:
-    T, KV, D = _heads3(k, "k")
-    _need(_heads3(v, "v") == (T, KV, D), "v must be [T, H_kv, D] like k")
-    _vector(positions, torch.int64, T, "positions")
-    _vector(qsl, torch.int32, 1, "qsl")
-    B = qsl.numel() - 1
-    _need(_table(block_table).shape[0] >= B, "block_table needs a row for each sequence")
-    _pages2(cache, "cache")
+    T, KV, D, k0, k1 = _heads3(k, "k")
+    Tv, KVv, Dv, v0, v1 = _heads3(v, "v")
+    if T != Tv or KV != KVv or D != Dv:
+        _refuse("v must be [T, H_kv, D] like k")
+    pos, seqs = _vector(positions, torch.int64, T, "positions"), _vector(qsl, torch.int32, 1, "qsl")
+    B = qsl.shape[0] - 1
+    c, c0, pages = _bytes2(cache, "cache")
+    s = s0 = 0
     if summary is not None:
-        _need(_pages2(summary, "summary").shape[0] >= cache.shape[0], "summary needs a record for each page")
-    return ((k.data_ptr(), _st(k, 0), _st(k, 1), v.data_ptr(), _st(v, 0), _st(v, 1), T, KV, D),
-            (positions.data_ptr(), qsl.data_ptr(), B, int(max_query_len), block_table.data_ptr(), _st(block_table, 0),
-             block_table.shape[1], cache.data_ptr(), _st(cache, 0), cache.shape[0], _ptr(summary),
-             0 if summary is None else _st(summary, 0)))
+        s, s0, records = _bytes2(summary, "summary")
+        if records < pages:
+            _refuse("summary needs a record for each page")
+    return ((k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, T, KV, D),
+            (pos, seqs, B, max_query_len, *_table(block_table, B), c, c0, pages, s, s0))
 
 
 def gqa_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, qsl: torch.Tensor, max_query_len: int,
@@ -1208,48 +1251,49 @@ def gqa_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_w: torch.T
     """``qk_norm_rope`` of q and k and ``gqa_append`` of the prepared keys and
     ``v`` in one launch, same bytes; returns the prepared ``q``."""
     dev = _gqa_device(q, k, v, q_w, k_w, cos_sin, positions, qsl, block_table, cache, summary)
-    T, H, D = _heads3(q, "q")
-    _need(k.dim() == 3 and k.shape[0] == T and k.shape[2] == D, "k must be [T, H_kv, D] like q")
+    T, H, D, q0, q1 = _heads3(q, "q")
     head, tail = _append_args(k, v, positions, qsl, max_query_len, block_table, cache, summary)
-    weights, rope = _norm_args(q_w, k_w, D, cos_sin, rope_offset, interleaved)
-    q_out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    _gqa_call(dev, "ekv_gqa_prologue", q.data_ptr(), _st(q, 0), _st(q, 1), H, *head, *weights, float(eps), *rope, *tail,
-              q_out.data_ptr())
+    if head[6] != T or head[8] != D:
+        _refuse("k must be [T, H_kv, D] like q")
+    norm = _norm_args(q_w, k_w, D, eps, cos_sin, rope_offset, interleaved)
+    q_out = q.new_empty((T, H, D))
+    _gqa_call(dev, "ekv_gqa_prologue", q.data_ptr(), q0, q1, H, *head, *norm, *tail, q_out.data_ptr())
     return q_out
 
 
-def _gqa_attn_args(q, cache, kv_heads, block_table, positions, out, lse, sinks) -> tuple:
-    T, H, D = _heads3(q, "q")
-    _need(kv_heads > 0 and H % kv_heads == 0, "heads must be a multiple of kv_heads")
-    _pages2(cache, "cache")
-    _table(block_table)
-    _vector(positions, torch.int64, T, "positions")
-    _need(out.dtype == torch.bfloat16 and out.shape == (T, H, D) and out.stride(2) == 1, "out bf16 [T, H, D]")
+def _gqa_attn_args(q, cache, kv_heads, block_table, seqs, positions, out, lse, sinks) -> tuple:
+    T, H, D, q0, q1 = _heads3(q, "q")
+    if kv_heads <= 0 or H % kv_heads:
+        _refuse("heads must be a multiple of kv_heads")
+    To, Ho, Do, o0, o1 = _heads3(out, "out")
+    if To != T or Ho != H or Do != D:
+        _refuse("out bf16 [T, H, D] like q")
+    l = l0 = 0
     if lse is not None:
-        _need(lse.dtype == torch.float32 and lse.shape == (T, H) and (H <= 1 or lse.stride(1) == 1), "lse fp32 [T, H]")
-    if sinks is not None:
-        _vector(sinks, torch.float32, H, "sinks")
-    return ((q.data_ptr(), _st(q, 0), _st(q, 1), T, H, int(kv_heads), D, cache.data_ptr(), _st(cache, 0),
-             cache.shape[0], block_table.data_ptr(), _st(block_table, 0), block_table.shape[1], positions.data_ptr()),
-            (out.data_ptr(), _st(out, 0), _st(out, 1), _ptr(lse), 0 if lse is None else _st(lse, 0)))
+        if lse.dtype is not torch.float32 or lse.dim() != 2 or lse.shape != (T, H) or (H > 1 and lse.stride(1) != 1):
+            _refuse("lse fp32 [T, H]")
+        l, l0 = lse.data_ptr(), lse.stride(0)
+    s = None if sinks is None else _vector(sinks, torch.float32, H, "sinks")
+    return (T, H, D, (q.data_ptr(), q0, q1, T, H, kv_heads, D, *_bytes2(cache, "cache"), *_table(block_table, seqs),
+                      _vector(positions, torch.int64, T, "positions")), s, (out.data_ptr(), o0, o1, l, l0))
 
 
-def _gqa_workspace(workspace, need: int, dev) -> tuple:
+def _gqa_workspace(workspace, need: int, like: torch.Tensor) -> tuple:
+    """(address, bytes, the tensor) of the call's workspace."""
     if workspace is None:
         if not need:
-            return None, (None, 0)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    _need(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.numel() >= need,
-          f"workspace too small: {workspace.numel()} < {need} bytes")
-    return workspace, (workspace.data_ptr(), workspace.numel())
+            return None, 0, None
+        workspace = like.new_empty(need, dtype=torch.uint8)
+    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+        _refuse(f"workspace too small, or not contiguous uint8: {workspace.numel()} < {need} bytes")
+    return workspace.data_ptr(), workspace.numel(), workspace
 
 
 def gqa_attention_workspace(num_tokens: int, num_seqs: int, max_query_len: int, max_len: int, heads: int,
                             kv_heads: int, dim: int, device, window: int = 0) -> torch.Tensor:
     """Workspace of ``gqa_attention`` for calls of exactly these sizes."""
-    n = _lib.load().ekv_gqa_attention_workspace_size(num_tokens, num_seqs, max_query_len, max_len, heads, kv_heads, dim,
-                                                     window)
-    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=device)
+    n = _attention_bytes(num_tokens, num_seqs, max_query_len, max_len, heads, kv_heads, dim, window)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
 def gqa_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, block_table: torch.Tensor,
@@ -1261,15 +1305,22 @@ def gqa_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, block_tab
     ``window`` of them where it is not 0; ``sinks`` enter the denominator only.
     Rows that see nothing get zeros and -inf, rows of no sequence stay."""
     dev = _gqa_device(q, cache, block_table, positions, qsl, out, lse, sinks, workspace)
-    head, tail = _gqa_attn_args(q, cache, kv_heads, block_table, positions, out, lse, sinks)
-    _vector(qsl, torch.int32, 1, "qsl")
-    B, T, H, D = qsl.numel() - 1, *q.shape
-    _need(block_table.shape[0] >= B, "block_table needs a row for each sequence")
-    need = _lib.load().ekv_gqa_attention_workspace_size(T, B, int(max_query_len), int(max_len), H, int(kv_heads), D,
-                                                        int(window))
-    workspace, ws = _gqa_workspace(workspace, need, dev)
-    _gqa_call(dev, "ekv_gqa_attention", *head, qsl.data_ptr(), B, int(max_query_len), int(max_len), int(window),
-              _ptr(sinks), float(scale), *tail, *ws)
+    seqs = _vector(qsl, torch.int32, 1, "qsl")
+    B = qsl.shape[0] - 1
+    T, H, D, head, sink, tail = _gqa_attn_args(q, cache, kv_heads, block_table, B, positions, out, lse, sinks)
+    ws, ws_bytes, workspace = _gqa_workspace(
+        workspace, _attention_bytes(T, B, max_query_len, max_len, H, kv_heads, D, window), q)
+    _gqa_call(dev, "ekv_gqa_attention", *head, seqs, B, max_query_len, max_len, window, sink, scale, *tail, ws, ws_bytes)
+
+
+def _block_lists(blocks, T: int, kv_heads: int) -> tuple:
+    if blocks.dtype is not torch.int32 or blocks.dim() != 3:
+        _refuse("blocks int32 [T, H_kv, n]")
+    t, h, n = blocks.shape
+    s0, s1, s2 = blocks.stride()
+    if t != T or h != kv_heads or (s2 != 1 and n > 1):
+        _refuse("blocks int32 [T, H_kv, n] with unit stride in a list")
+    return blocks.data_ptr(), s0, s1, n
 
 
 def gqa_block_select(q: torch.Tensor, summary: torch.Tensor, kv_heads: int, block_table: torch.Tensor,
@@ -1279,25 +1330,20 @@ def gqa_block_select(q: torch.Tensor, summary: torch.Tensor, kv_heads: int, bloc
     the largest score against their mean keys, ascending, -1 behind them; the
     first ``keep_first`` and the last ``keep_last`` pages come before others."""
     dev = _gqa_device(q, summary, block_table, positions, req_ids, blocks)
-    T, H, D = _heads3(q, "q")
-    _need(kv_heads > 0 and H % kv_heads == 0, "heads must be a multiple of kv_heads")
-    _pages2(summary, "summary")
-    _table(block_table)
-    _vector(positions, torch.int64, T, "positions")
-    _vector(req_ids, torch.int32, T, "req_ids")
-    _need(blocks.dtype == torch.int32 and blocks.dim() == 3 and blocks.shape[:2] == (T, kv_heads)
-          and (blocks.shape[2] <= 1 or blocks.stride(2) == 1), "blocks int32 [T, H_kv, n]")
-    _gqa_call(dev, "ekv_gqa_block_select", q.data_ptr(), _st(q, 0), _st(q, 1), T, H, int(kv_heads), D,
-              summary.data_ptr(), _st(summary, 0), summary.shape[0], block_table.data_ptr(), _st(block_table, 0),
-              block_table.shape[1], positions.data_ptr(), req_ids.data_ptr(), block_table.shape[0], int(max_len),
-              int(keep_first), int(keep_last), blocks.data_ptr(), _st(blocks, 0), _st(blocks, 1), blocks.shape[2])
+    T, H, D, q0, q1 = _heads3(q, "q")
+    if kv_heads <= 0 or H % kv_heads:
+        _refuse("heads must be a multiple of kv_heads")
+    _gqa_call(dev, "ekv_gqa_block_select", q.data_ptr(), q0, q1, T, H, kv_heads, D, *_bytes2(summary, "summary"),
+              *_table(block_table, 0), _vector(positions, torch.int64, T, "positions"),
+              _vector(req_ids, torch.int32, T, "req_ids"), block_table.shape[0], max_len, keep_first, keep_last,
+              *_block_lists(blocks, T, kv_heads))
 
 
 def gqa_block_attention_workspace(num_tokens: int, heads: int, kv_heads: int, dim: int, num_blocks: int,
                                   device) -> torch.Tensor:
     """Workspace of ``gqa_block_attention`` for calls of exactly these sizes."""
-    n = _lib.load().ekv_gqa_block_attention_workspace_size(num_tokens, heads, kv_heads, dim, num_blocks)
-    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=device)
+    n = _block_attention_bytes(num_tokens, heads, kv_heads, dim, num_blocks)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
 def gqa_block_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, block_table: torch.Tensor,
@@ -1307,13 +1353,8 @@ def gqa_block_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, blo
     """``gqa_attention`` over the pages that ``blocks [T, H_kv, n]`` lists for
     each row and kv head (``gqa_block_select``; negative entries skipped)."""
     dev = _gqa_device(q, cache, block_table, positions, req_ids, blocks, out, lse, sinks, workspace)
-    head, tail = _gqa_attn_args(q, cache, kv_heads, block_table, positions, out, lse, sinks)
-    T, H, D = q.shape
-    _vector(req_ids, torch.int32, T, "req_ids")
-    _need(blocks.dtype == torch.int32 and blocks.dim() == 3 and blocks.shape[:2] == (T, kv_heads)
-          and (blocks.shape[2] <= 1 or blocks.stride(2) == 1), "blocks int32 [T, H_kv, n]")
-    n = blocks.shape[2]
-    need = _lib.load().ekv_gqa_block_attention_workspace_size(T, H, int(kv_heads), D, n)
-    workspace, ws = _gqa_workspace(workspace, need, dev)
-    _gqa_call(dev, "ekv_gqa_block_attention", *head, req_ids.data_ptr(), block_table.shape[0], blocks.data_ptr(),
-              _st(blocks, 0), _st(blocks, 1), n, _ptr(sinks), float(scale), *tail, *ws)
+    T, H, D, head, sink, tail = _gqa_attn_args(q, cache, kv_heads, block_table, 0, positions, out, lse, sinks)
+    lists = _block_lists(blocks, T, kv_heads)
+    ws, ws_bytes, workspace = _gqa_workspace(workspace, _block_attention_bytes(T, H, kv_heads, D, lists[3]), q)
+    _gqa_call(dev, "ekv_gqa_block_attention", *head, _vector(req_ids, torch.int32, T, "req_ids"), block_table.shape[0],
+              *lists, sink, scale, *tail, ws, ws_bytes)
