@@ -85,6 +85,151 @@ __device__ __forceinline__ void store_lse(const GqaAttnArgs& a, int64_t t, int h
   if (a.lse) a.lse[t * a.lse_stride + hq] = l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
+// Rows of a wave's NT tiles of 16 queries: what each lane's row sees.
+template <int NT>
+struct RowRange {
+  int pos[NT], lo[NT];        // the row sees lo .. pos
+  int pmax, pmin, pany;       // of the wave's rows: last token, first of rows that see any, first of all
+};
+
+// Scores x (token 16 j + 4 g + i of the page, row n) -> weights around the
+// rows' references m, as the B operand of the product with V, and their sums.
+// kscale > 0 takes a raw score to log2 units.  The references move only when a
+// score exceeds one by kSlack: weights stay below 2^kSlack, and most pages
+// need no maximum across lanes.  Masks are selects without branches.
+template <int NT, int DT>
+__device__ __forceinline__ void softmax_page(f32x4 (&x)[NT][4], float kscale, bool whole, int first, int g,
+                                             const RowRange<NT>& r, float (&m)[NT], float (&l)[NT],
+                                             f32x4 (&o)[NT][DT], bf16x8 (&w)[NT][2]) {
+  if (!whole) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int from = r.lo[nt] - first - 4 * g, to = r.pos[nt] - first - 4 * g;  // seen: from <= 16 j + i <= to
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = 16 * j + i;
+          x[nt][j][i] = (at >= from) & (at <= to) ? x[nt][j][i] : -__builtin_inff();
+        }
+      }
+    }
+  }
+  float top[NT], most = kNone;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    top[nt] = x[nt][0][0];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[nt] = fmaxf(top[nt], x[nt][j][i]);
+    }
+    top[nt] *= kscale;
+    most = fmaxf(most, top[nt] - m[nt]);
+  }
+  if (__any(most > kSlack)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float t = fmaxf(top[nt], m[nt]);
+      t = fmaxf(t, __shfl_xor(t, 16, 64));
+      t = fmaxf(t, __shfl_xor(t, 32, 64));
+      const float f = __builtin_amdgcn_exp2f(m[nt] - t);
+      m[nt] = t;
+      l[nt] *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[nt][d] *= f;
+    }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[nt][j][i], kscale, -m[nt]));
+        l[nt] += y;
+        w[nt][j >> 1][4 * (j & 1) + i] = static_cast<__bf16>(y);
+      }
+    }
+  }
+}
+
+// The bytes of V group g that belong to tokens low .. last of the page at
+// `first`: what lies outside may be anything, NaN codes too.
+__device__ __forceinline__ uint4 v_keep(int first, int low, int last, int g) {
+  uint32_t keep[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    keep[t] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int tok = first + 16 * t + 4 * g + i;
+      keep[t] |= (tok <= last) & (tok >= low) ? 0xffu << (8 * i) : 0u;
+    }
+  }
+  return make_uint4(keep[0], keep[1], keep[2], keep[3]);
+}
+
+__device__ __forceinline__ uint4 and4(uint4 a, uint4 b) { return make_uint4(a.x & b.x, a.y & b.y, a.z & b.z, a.w & b.w); }
+
+// q of NT tiles of rows r0 .. (flattened (token, head of the group) from token
+// t0 on) as the B operand, and what the rows see.
+template <int D, int NT>
+__device__ __forceinline__ void load_rows(const GqaAttnArgs& a, int t0, int h, int r0, int rows, int n, int g,
+                                          bf16x8 (&q)[NT][D / 64][2], RowRange<NT>& rr) {
+  rr.pmax = -1, rr.pmin = 0x7fffffff, rr.pany = 0x7fffffff;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = r0 + 16 * nt + n;
+    const bool have = r < rows;
+    const int tok = have ? r / a.group : 0, hq = h * a.group + (have ? r - tok * a.group : 0);
+    rr.pos[nt] = 0x7fffffff;  // no row: unmasked zeros, never stored
+    if (have) {
+      const int p = static_cast<int>(min(max(a.positions[t0 + tok], static_cast<int64_t>(-1)),
+                                         static_cast<int64_t>(0x3fffffff)));
+      rr.pos[nt] = p;
+      rr.pmax = max(rr.pmax, p);
+      rr.pany = min(rr.pany, p);
+      if (p >= 0) rr.pmin = min(rr.pmin, p);
+    }
+    rr.lo[nt] = a.window ? rr.pos[nt] - a.window + 1 : 0;
+    const uint16_t* src = a.q + (t0 + tok) * a.q_tok_stride + hq * a.q_head_stride + 16 * g;
+#pragma unroll
+    for (int s = 0; s < D / 64; ++s) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        q[nt][s][u] = bf16x8{};
+        if (have) q[nt][s][u] = load_q8(src + 64 * s + 8 * u, a.q_aligned);
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) {
+    rr.pmax = max(rr.pmax, __shfl_xor(rr.pmax, m, 64));
+    rr.pmin = min(rr.pmin, __shfl_xor(rr.pmin, m, 64));
+    rr.pany = min(rr.pany, __shfl_xor(rr.pany, m, 64));
+  }
+  rr.pmax = __builtin_amdgcn_readfirstlane(rr.pmax);
+  rr.pmin = __builtin_amdgcn_readfirstlane(rr.pmin);
+  rr.pany = __builtin_amdgcn_readfirstlane(rr.pany);
+}
+
+// Lane i's page at logical index lp (-1: none): its place in the cache (-1:
+// skipped) and its scales.
+__device__ __forceinline__ int page_of(const GqaAttnArgs& a, const int32_t* bt, int h, int dim, int lp, int pmax,
+                                       float& ks, float& vs) {
+  int page = -1;
+  if (lp >= 0 && lp < a.bt_width && lp * static_cast<int64_t>(kPageTokens) <= pmax) page = bt[lp];
+  if (page >= a.num_pages) page = -1;
+  ks = vs = 0.0f;
+  if (page >= 0) {
+    const float* sc = reinterpret_cast<const float*>(a.cache + page * a.page_stride +
+                                                     2ll * a.kv_heads * kPageTokens * dim) + h;
+    ks = sc[0] * a.scale_log2, vs = sc[a.kv_heads];
+  }
+  return page;
+}
+
 // ---------------------------------------------------------------------------
 // Few rows a kv head: one workgroup per (16 NT rows, kv head, range of pages).
 // Each of its 4 waves takes every fourth page of the range through registers,
@@ -113,41 +258,11 @@ __global__ void __launch_bounds__(256) gqa_decode_kernel(GqaAttnArgs a) {
   }
   const int r0 = tile * 16 * NT;
   if (r0 >= rows) return;
-  int pos[NT], lo[NT], pmax = -1, pmin = 0x7fffffff, pany = 0x7fffffff;
+  RowRange<NT> rr;
   bf16x8 q[NT][S][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = r0 + 16 * nt + n;
-    const bool have = r < rows;
-    const int tok = have ? r / a.group : 0, hq = h * a.group + (have ? r - tok * a.group : 0);
-    pos[nt] = 0x7fffffff;  // no row: unmasked zeros, never stored
-    if (have) {
-      pos[nt] = static_cast<int>(min(max(a.positions[t0 + tok], -1ll), 0x3fffffffll));
-      pmax = max(pmax, pos[nt]);
-      pany = min(pany, pos[nt]);
-      if (pos[nt] >= 0) pmin = min(pmin, pos[nt]);
-    }
-    lo[nt] = a.window ? pos[nt] - a.window + 1 : 0;  // the row sees lo .. pos
-    const uint16_t* src = a.q + (t0 + tok) * a.q_tok_stride + hq * a.q_head_stride + 16 * g;
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        q[nt][s][u] = bf16x8{};
-        if (have) q[nt][s][u] = load_q8(src + 64 * s + 8 * u, a.q_aligned);
-      }
-    }
-  }
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) {
-    pmax = max(pmax, __shfl_xor(pmax, m, 64));
-    pmin = min(pmin, __shfl_xor(pmin, m, 64));
-    pany = min(pany, __shfl_xor(pany, m, 64));
-  }
-  pmax = __builtin_amdgcn_readfirstlane(pmax);
-  pmin = __builtin_amdgcn_readfirstlane(pmin);
-  pany = __builtin_amdgcn_readfirstlane(pany);
-  const int low = a.window && pmax >= 0 ? max(pmin - a.window + 1, 0) : 0;  // first token any row sees
+  load_rows<D, NT>(a, t0, h, r0, rows, n, g, q, rr);
+  const int pmax = rr.pmax;
+  const int low = a.window && pmax >= 0 ? max(rr.pmin - a.window + 1, 0) : 0;  // first token any row sees
 
   int pb, pe;
   if (LIST) {
@@ -170,16 +285,10 @@ __global__ void __launch_bounds__(256) gqa_decode_kernel(GqaAttnArgs a) {
   for (int p0 = pb + wave; p0 < pe; p0 += 256) {
     // lane i: the wave's i-th page of the next 64, its place and its scales
     const int e = p0 + 4 * lane;
-    int lp = -1, page = -1;
-    float ks = 0.0f, vs = 0.0f;
+    int lp = -1;
+    float ks, vs;
     if (e < pe) lp = LIST ? a.ids[t0 * a.ids_tok_stride + h * a.ids_head_stride + e] : e;
-    if (lp >= 0 && lp < a.bt_width && lp * static_cast<int64_t>(kPageTokens) <= pmax) page = bt[lp];
-    if (page >= a.num_pages) page = -1;
-    if (page >= 0) {
-      const float* sc = reinterpret_cast<const float*>(a.cache + page * a.page_stride +
-                                                       2ll * a.kv_heads * kPageTokens * D) + h;
-      ks = sc[0], vs = sc[a.kv_heads];
-    }
+    const int page = page_of(a, bt, h, D, lp, pmax, ks, vs);
     uint64_t todo = __ballot(page >= 0);
     if (!todo) continue;
     uint4 kr[4][S], vr[DT];
@@ -200,7 +309,7 @@ __global__ void __launch_bounds__(256) gqa_decode_kernel(GqaAttnArgs a) {
       const uint8_t* ng =
           a.cache + static_cast<int64_t>(__builtin_amdgcn_readlane(page, next < 0 ? at : next)) * a.page_stride;
       const int first = __builtin_amdgcn_readlane(lp, at) * kPageTokens;
-      const float kscale = lane_value(ks, at) * a.scale_log2, vscale = lane_value(vs, at);
+      const float kscale = lane_value(ks, at), vscale = lane_value(vs, at);
 
       f32x4 x[NT][4] = {};
 #pragma unroll
@@ -223,85 +332,13 @@ __global__ void __launch_bounds__(256) gqa_decode_kernel(GqaAttnArgs a) {
         }
       }
 
-      const bool whole = first + kPageTokens - 1 <= pany && (!a.window || first > pmax - a.window);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[nt][j] *= kscale;
-      }
-      if (!whole) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int from = lo[nt] - first - 4 * g, to = pos[nt] - first - 4 * g;  // seen: from <= 16 j + i <= to
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int at = 16 * j + i;
-              x[nt][j][i] = (at >= from) & (at <= to) ? x[nt][j][i] : -__builtin_inff();
-            }
-          }
-        }
-      }
-      float most = kNone;  // of x over its reference
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float top = x[nt][0][0];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, x[nt][j][i]);
-        }
-        most = fmaxf(most, top - m[nt]);
-      }
-      if (__any(most > kSlack)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float top = m[nt];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, x[nt][j][i]);
-          }
-          top = fmaxf(top, __shfl_xor(top, 16, 64));
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float f = __builtin_amdgcn_exp2f(m[nt] - top);
-          m[nt] = top;
-          l[nt] *= f;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[nt][d] *= f;
-        }
-      }
+      const bool whole = first + kPageTokens - 1 <= rr.pany && (!a.window || first > pmax - a.window);
       bf16x8 w[NT][2];
+      softmax_page<NT, DT>(x, kscale, whole, first, g, rr, m, l, o, w);
+      if (!whole) {
+        const uint4 keep = v_keep(first, low, pmax, g);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float y = __builtin_amdgcn_exp2f(x[nt][j][i] - m[nt]);
-            l[nt] += y;
-            w[nt][j >> 1][4 * (j & 1) + i] = static_cast<__bf16>(y);
-          }
-        }
-      }
-      if (!whole) {  // bytes behind the last token, or before the first, may be anything
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          uint32_t keep = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int tok = first + 16 * t + 4 * g + i;
-            if (tok <= pmax && tok >= low) keep |= 0xffu << (8 * i);
-          }
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            if (t == 0) vr[d].x &= keep;
-            else if (t == 1) vr[d].y &= keep;
-            else if (t == 2) vr[d].z &= keep;
-            else vr[d].w &= keep;
-          }
-        }
+        for (int d = 0; d < DT; ++d) vr[d] = and4(vr[d], keep);
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
@@ -359,6 +396,150 @@ __global__ void __launch_bounds__(256) gqa_decode_kernel(GqaAttnArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows a kv head: one workgroup per (128 rows, kv head, range of pages).
+// Its 4 waves hold 32 rows each and share every page: each wave brings a
+// quarter of it, converted to bf16 once, into LDS in the order of the operands
+// (1 KB reads of 64 consecutive 16-byte pieces), while the page before is
+// multiplied.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaAttnArgs a) {
+  constexpr int S = D / 64, DT = D / 16, VT = DT / 4, NT = 2;
+  constexpr int kHalf = (8 * S + 2 * DT) * 64;  // 16-byte pieces of a page: K, then V
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  bf16x8* const buf = reinterpret_cast<bf16x8*>(smem);
+  __shared__ int ranges[4][2];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int unit = static_cast<int>(blockIdx.x) % a.units, split = static_cast<int>(blockIdx.x) / a.units;
+  const int h = unit % a.kv_heads, rest = unit / a.kv_heads;
+  const int b = rest % a.num_seqs, tile = a.tiles - 1 - rest / a.num_seqs;  // the longest rows first
+  const int t0 = a.qsl[b];
+  const int rows = (min(a.qsl[b + 1], a.num_tokens) - t0) * a.group;
+  if (t0 < 0 || tile * 128 >= rows) return;
+  const int r0 = tile * 128 + 32 * wave;
+  RowRange<NT> rr;
+  bf16x8 q[NT][S][2];
+  load_rows<D, NT>(a, t0, h, r0, rows, n, g, q, rr);
+  if (lane == 0) ranges[wave][0] = rr.pmax, ranges[wave][1] = rr.pmin;
+  __syncthreads();
+  int pmax = -1, pmin = 0x7fffffff;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) pmax = max(pmax, ranges[w][0]), pmin = min(pmin, ranges[w][1]);
+  pmax = __builtin_amdgcn_readfirstlane(pmax);
+  pmin = __builtin_amdgcn_readfirstlane(pmin);
+  const int low = a.window && pmax >= 0 ? max(pmin - a.window + 1, 0) : 0;
+  const int wave_low = a.window && rr.pmax >= 0 ? max(rr.pmin - a.window + 1, 0) : 0;
+  const int last = pmax < 0 ? 0 : min(pmax / kPageTokens + 1, a.bt_width);
+  const int pb = low / kPageTokens + split * a.split_pages;
+  const int pe = split == a.splits - 1 ? last : min(pb + a.split_pages, last);
+
+  f32x4 o[NT][DT] = {};
+  float m[NT], l[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) m[nt] = kNone, l[nt] = 0.0f;
+
+  // this wave's quarter of a page: tokens 16 wave .. of K, channels D / 4 wave .. of V
+  const int64_t k_at = static_cast<int64_t>(h) * kPageTokens * D + (16 * wave + n) * D + 16 * g;
+  const int64_t v_at = static_cast<int64_t>(a.kv_heads + h) * kPageTokens * D + (D / 4 * wave + n) * kPageTokens + 16 * g;
+  const int32_t* bt = a.block_table + b * a.bt_stride;
+  uint4 kr[S], vr[VT];
+
+  for (int p0 = pb; p0 < pe; p0 += 64) {
+    float ks, vs;
+    const int page = page_of(a, bt, h, D, p0 + lane < pe ? p0 + lane : -1, pmax, ks, vs);
+    uint64_t todo = __ballot(page >= 0);
+    if (!todo) continue;
+    auto fetch = [&](int at) {
+      const uint8_t* pg = a.cache + static_cast<int64_t>(__builtin_amdgcn_readlane(page, at)) * a.page_stride;
+#pragma unroll
+      for (int s = 0; s < S; ++s) kr[s] = *reinterpret_cast<const uint4*>(pg + k_at + 64 * s);
+#pragma unroll
+      for (int i = 0; i < VT; ++i) vr[i] = *reinterpret_cast<const uint4*>(pg + v_at + 16 * i * kPageTokens);
+    };
+    auto stage = [&](int at, int half) {
+      bf16x8* const dst = buf + half * kHalf + lane;
+      const int first = (p0 + at) * kPageTokens;
+      const float vscale = lane_value(vs, at);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        dst[((wave * S + s) * 2) * 64] = fp8x8_to_bf16(kr[s].x, kr[s].y, 1.0f);
+        dst[((wave * S + s) * 2 + 1) * 64] = fp8x8_to_bf16(kr[s].z, kr[s].w, 1.0f);
+      }
+      if (first + kPageTokens - 1 > pmax || first < low) {
+        const uint4 keep = v_keep(first, low, pmax, g);
+#pragma unroll
+        for (int i = 0; i < VT; ++i) vr[i] = and4(vr[i], keep);
+      }
+#pragma unroll
+      for (int i = 0; i < VT; ++i) {
+        dst[(8 * S + (wave * VT + i) * 2) * 64] = fp8x8_to_bf16(vr[i].x, vr[i].y, vscale);
+        dst[(8 * S + (wave * VT + i) * 2 + 1) * 64] = fp8x8_to_bf16(vr[i].z, vr[i].w, vscale);
+      }
+    };
+    int at = __builtin_ctzll(todo), half = 0;
+    __syncthreads();  // the buffers of the 64 pages before
+    fetch(at);
+    stage(at, 0);
+    while (at >= 0) {
+      todo &= todo - 1;
+      const int next = todo ? __builtin_ctzll(todo) : -1;
+      __syncthreads();  // page `at` is whole in its half; the other half is read no more
+      if (next >= 0) fetch(next);
+      const int first = (p0 + at) * kPageTokens;
+      if (first <= rr.pmax && first + kPageTokens > wave_low) {
+        const bf16x8* const src = buf + half * kHalf + lane;
+        f32x4 x[NT][4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int s = 0; s < 2 * S; ++s) {
+            const bf16x8 k = src[(j * 2 * S + s) * 64];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              x[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[nt][s >> 1][s & 1], x[nt][j], 0, 0, 0);
+          }
+        }
+        const bool whole = first + kPageTokens - 1 <= rr.pany && (!a.window || first > rr.pmax - a.window);
+        bf16x8 w[NT][2];
+        softmax_page<NT, DT>(x, lane_value(ks, at), whole, first, g, rr, m, l, o, w);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const bf16x8 v = src[(8 * S + 2 * d + u) * 64];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[nt][u], o[nt][d], 0, 0, 0);
+          }
+        }
+      }
+      if (next >= 0) stage(next, half ^ 1);
+      at = next, half ^= 1;
+    }
+  }
+
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    l[nt] += __shfl_xor(l[nt], 16, 64);
+    l[nt] += __shfl_xor(l[nt], 32, 64);
+    const int r = r0 + 16 * nt + n;
+    if (r >= rows) continue;
+    const int64_t t = t0 + r / a.group;
+    const int hq = h * a.group + r % a.group;
+    const int64_t at = (static_cast<int64_t>(split) * a.num_tokens + t) * a.heads + hq;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      if (a.splits == 1) store_out4(a, t, hq, 16 * d + 4 * g, o[nt][d], m[nt], l[nt]);
+      else *reinterpret_cast<f32x4*>(a.ws_o + at * D + 16 * d + 4 * g) = o[nt][d];
+    }
+    if (g == 0) {
+      if (a.splits == 1) store_lse(a, t, hq, m[nt], l[nt]);
+      else a.ws_ml[at] = make_float2(m[nt], l[nt]);
+    }
+  }
+}
+
 // Joins the splits: one wave per (token, head), lane s the s-th split's weight.
 template <int D, bool LIST>
 __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a) {
@@ -399,30 +580,40 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a) {
 // Host side
 // ---------------------------------------------------------------------------
 struct GqaPlan {
-  int row_tiles;  // 16-row tiles a workgroup takes
+  int row_tiles;  // 16-row tiles of a workgroup: 1, 2, 4 in every wave, or 8 over its four waves
   int tiles, splits, split_pages;
   int64_t units;
 };
 
-// seqs: sequences (dense) or tokens (selected blocks); rows: query rows a kv head has in each.
-static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int kv_heads, int dim, int64_t pages) {
+// seqs: sequences (dense) or tokens (selected blocks); rows: query rows a kv
+// head has in each; pages(n): the most pages that n consecutive rows see.
+template <typename Pages>
+static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int kv_heads, int dim, bool list, Pages pages_of) {
   GqaPlan p{};
   const int most = dim == 256 ? 1 : dim == 128 ? 2 : 4;
-  p.row_tiles = rows <= 16 || most == 1 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
+  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : rows <= 64 || list ? most : 8;
   p.tiles = static_cast<int>((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
   p.units = seqs * kv_heads * p.tiles;
-  pages = std::max<int64_t>(pages, 1);
-  int64_t splits = std::min<int64_t>({(1024 + p.units - 1) / std::max<int64_t>(p.units, 1), (pages + 3) / 4, kMaxSplits});
+  const int64_t pages = std::max<int64_t>(pages_of(std::min<int64_t>(rows, 16 * p.row_tiles)), 1);
+  const int64_t want = p.row_tiles == 8 ? 512 : 1024;
+  int64_t splits = std::min<int64_t>({(want + p.units - 1) / std::max<int64_t>(p.units, 1), (pages + 3) / 4, kMaxSplits});
   splits = std::max<int64_t>(splits, 1);
   p.split_pages = static_cast<int>((pages + splits - 1) / splits);
   p.splits = static_cast<int>((pages + p.split_pages - 1) / p.split_pages);
   return p;
 }
 
-static int64_t dense_pages(int64_t max_len, int64_t max_query_len, int64_t window) {
-  int64_t pages = (max_len + kPageTokens - 1) / kPageTokens;
-  if (window) pages = std::min(pages, (window + max_query_len - 2) / kPageTokens + 2);
-  return pages;
+static GqaPlan dense_plan(int64_t seqs, int64_t max_rows, int group, int kv_heads, int dim, int64_t max_len,
+                          int64_t window) {
+  return gqa_plan(seqs, max_rows * group, kv_heads, dim, false, [&](int64_t rows) {
+    const int64_t all = (max_len + kPageTokens - 1) / kPageTokens;
+    const int64_t tokens = (rows + group - 1) / group + 1;  // of a tile that begins inside one
+    return window ? std::min(all, (window + tokens - 2) / kPageTokens + 2) : all;
+  });
+}
+
+static GqaPlan block_plan(int64_t num_tokens, int group, int kv_heads, int dim, int64_t num_blocks) {
+  return gqa_plan(num_tokens, group, kv_heads, dim, true, [&](int64_t) { return num_blocks; });
 }
 
 static int64_t plan_bytes(const GqaPlan& p, int64_t num_tokens, int64_t heads, int64_t dim) {
@@ -434,6 +625,15 @@ static int launch_decode(const GqaAttnArgs& a, int row_tiles, hipStream_t s) {
   const int64_t blocks = static_cast<int64_t>(a.units) * a.splits;
   EKV_CHECK(blocks < (int64_t{1} << 31), "too many rows for one call");
   const dim3 grid(static_cast<uint32_t>(blocks));
+  if constexpr (!LIST) {
+    if (row_tiles == 8) {
+      constexpr int kBytes = 2 * (D / 8 + D / 8) * 64 * 16;
+      if (kBytes >= 65536)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(gqa_prefill_kernel<D>),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+      gqa_prefill_kernel<D><<<grid, 256, kBytes, s>>>(a);
+    }
+  }
   if (row_tiles == 1) gqa_decode_kernel<D, 1, LIST><<<grid, 256, 0, s>>>(a);
   if constexpr (D <= 128) {
     if (row_tiles == 2) gqa_decode_kernel<D, 2, LIST><<<grid, 256, 0, s>>>(a);
@@ -475,6 +675,7 @@ static int attn_args(GqaAttnArgs& a, const uint16_t* q, int64_t q_tok_stride, in
   EKV_CHECK(gqa_dim(dim), "dim must be 64, 128 or 256");
   EKV_CHECK(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "heads must be a multiple of kv_heads");
   EKV_CHECK(num_tokens >= 0 && num_seqs >= 0 && num_pages >= 0 && bt_width >= 0, "negative sizes");
+  EKV_CHECK(scale > 0.0f, "scale must be positive");
   a = GqaAttnArgs{};
   if (!num_tokens || !num_seqs) return kOk;
   EKV_CHECK(q && cache && block_table && positions && out, "null pointer");
@@ -505,8 +706,7 @@ extern "C" int64_t ekv_gqa_attention_workspace_size(int32_t num_tokens, int32_t 
       window < 0)
     return 0;
   const int64_t rows = std::min(max_query_len, num_tokens);
-  return plan_bytes(gqa_plan(num_seqs, rows * (heads / kv_heads), kv_heads, dim,
-                             dense_pages(std::max(max_len, 0), rows, window)),
+  return plan_bytes(dense_plan(num_seqs, rows, heads / kv_heads, kv_heads, dim, std::max(max_len, 0), window),
                     num_tokens, heads, dim);
 }
 
@@ -528,14 +728,14 @@ extern "C" int ekv_gqa_attention(const uint16_t* q, int64_t q_tok_stride, int64_
   EKV_CHECK(qsl, "null pointer");
   a.qsl = qsl, a.window = window;
   const int64_t rows = std::min(max_query_len, num_tokens);
-  return launch_attn<false>(a, gqa_plan(num_seqs, rows * a.group, kv_heads, dim, dense_pages(max_len, rows, window)),
-                            dim, workspace, workspace_bytes, stream);
+  return launch_attn<false>(a, dense_plan(num_seqs, rows, a.group, kv_heads, dim, max_len, window), dim, workspace,
+                            workspace_bytes, stream);
 }
 
 extern "C" int64_t ekv_gqa_block_attention_workspace_size(int32_t num_tokens, int32_t heads, int32_t kv_heads,
                                                           int32_t dim, int32_t num_blocks) {
   if (num_tokens <= 0 || kv_heads <= 0 || heads < kv_heads || !gqa_dim(dim)) return 0;
-  return plan_bytes(gqa_plan(num_tokens, heads / kv_heads, kv_heads, dim, num_blocks), num_tokens, heads, dim);
+  return plan_bytes(block_plan(num_tokens, heads / kv_heads, kv_heads, dim, num_blocks), num_tokens, heads, dim);
 }
 
 extern "C" int ekv_gqa_block_attention(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride,
@@ -557,6 +757,6 @@ extern "C" int ekv_gqa_block_attention(const uint16_t* q, int64_t q_tok_stride, 
   EKV_CHECK(req_ids && (blocks || !num_blocks), "null pointer");
   a.req_ids = req_ids, a.ids = blocks, a.ids_tok_stride = blocks_tok_stride, a.ids_head_stride = blocks_head_stride;
   a.n_ids = num_blocks;
-  return launch_attn<true>(a, gqa_plan(num_tokens, a.group, kv_heads, dim, num_blocks), dim, workspace,
-                           workspace_bytes, stream);
+  return launch_attn<true>(a, block_plan(num_tokens, a.group, kv_heads, dim, num_blocks), dim, workspace, workspace_bytes,
+                           stream);
 }

@@ -1116,7 +1116,7 @@ def _heads3(t: torch.Tensor, what: str) -> tuple:
     """(T, heads, D, token stride, head stride) of bf16 rows; the stride of a
     dim of one entry, which no address depends on, is the packed one."""
     if t.dtype is not torch.bfloat16:
-        _refuse(f"{what}: expected bfloat16, got {t.dtype}")
+        _refuse(f"{what} bf16 [T, heads, D]: expected bfloat16, got {t.dtype}")
     if t.dim() != 3:
         _refuse(f"{what} [T, heads, D]")
     T, H, D = t.shape
