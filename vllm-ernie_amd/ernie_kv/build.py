@@ -52,7 +52,7 @@ SOURCES = {
     "ekv_mxfp4.hip": EXACT,
     "ekv_pages.hip": EXACT,
     "ekv_gqa_write.hip": EXACT,
-    "ekv_gqa_attn.hip": [],
+    "ekv_gqa_attn.hip": MFMA_VGPR,
     "ekv_gqa_select.hip": EXACT,
 }
 
