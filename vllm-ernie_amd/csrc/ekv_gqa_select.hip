@@ -15,15 +15,14 @@
 
 namespace ekv {
 
-constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 constexpr int kSelBins = 2048;
-constexpr int kSelMaxBlocks = 32768;  // keys of a row in LDS
+constexpr int kSelMaxBlocks = 32768;  // 16 waves of 32 keys a lane
 constexpr int kSelMaxGroup = 64;
 
 struct GqaSelectArgs {
   const uint16_t* q;
   int64_t q_tok_stride, q_head_stride;
-  int32_t num_tokens, heads, kv_heads, group;
+  int32_t q_aligned, num_tokens, heads, kv_heads, group;
   const uint8_t* summary;
   int64_t summary_stride, num_pages;
   const int32_t* block_table;
@@ -31,187 +30,260 @@ struct GqaSelectArgs {
   int32_t bt_width, num_seqs;
   const int64_t* positions;
   const int32_t* req_ids;
-  int32_t max_blocks;       // keys the LDS holds
+  int32_t max_blocks;       // pages that the lanes' keys hold
   int32_t n, keep_first, keep_last;
   int32_t* ids;
   int64_t ids_tok_stride, ids_head_stride;
 };
 
-// Counts of a workgroup's threads summed over all threads with a higher id.
-__device__ __forceinline__ uint32_t count_above(uint32_t v, uint32_t* tmp) {
-  const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
-  uint32_t s = v;
+__device__ __forceinline__ void load_q8(const uint16_t* p, bool aligned, float (&v)[8]) {
+  if (aligned) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint32_t o = __shfl_down(s, m, 64);
-    if (lane + m < 64) s += o;
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(ww[i] << 16);
+      v[2 * i + 1] = __uint_as_float(ww[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32(p[i]);
   }
-  if (lane == 0) tmp[wave] = s;
-  __syncthreads();
-  uint32_t above = s - v;
-  for (int w = wave + 1; w < kSelWaves; ++w) above += tmp[w];
-  __syncthreads();
-  return above;
 }
 
-// One workgroup per (token, kv head): the keys of all its pages in LDS, then
-// the n largest by three rounds of a histogram.
-template <int D>
-__global__ void __launch_bounds__(kSelThreads) gqa_block_select_kernel(GqaSelectArgs a) {
-  constexpr int S = D / 64;
-  extern __shared__ __attribute__((aligned(16))) uint32_t keys[];  // [max_blocks rounded up to 64]
-  __shared__ __attribute__((aligned(16))) int8_t qc[kSelMaxGroup * D];
-  __shared__ uint32_t bins[kSelBins];
-  __shared__ uint32_t tmp[kSelWaves], chunk[kSelMaxBlocks / 64 + 1];
-  __shared__ uint32_t found[2];
-  __shared__ float red[kSelWaves];
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-  const int h = static_cast<int>(blockIdx.x) % a.kv_heads;
-  const int64_t t = blockIdx.x / a.kv_heads;
+// One workgroup per (token, kv head).  Wave w holds the keys of the KPT * 64
+// pages from w * KPT * 64 on, one page a lane and chunk of 64; the n-th largest
+// key comes from three rounds of a histogram, and the chosen pages are written
+// in order by counts of the chunks before.
+template <int D, int WAVES, int KPT>
+__global__ void __launch_bounds__(64 * WAVES) gqa_block_select_kernel(GqaSelectArgs a) {
+  constexpr int S = D / 64, kThreads = 64 * WAVES, kRow = D + 16;  // padded rows: 16 of them in 16 bank groups
+  constexpr int kPer = kSelBins / kThreads;                        // bins a thread sums
+  constexpr bool kAhead = KPT <= 8;                                // pages asked for at entry
+  constexpr int kBuf = WAVES == 16 && (KPT > 8 || D == 256) ? 1 : 2;  // chunks of mean keys in registers
+  __shared__ __attribute__((aligned(16))) int8_t qc[kSelMaxGroup * kRow];
+  __shared__ __attribute__((aligned(16))) uint32_t bins[kSelBins];
+  __shared__ uint32_t sums[2][WAVES], found[3];
+  __shared__ float red[WAVES];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Eight tokens at a time, one an XCD (workgroup i runs on XCD i % 8): the
+  // heads of a page's record share cache lines, which its XCD's L2 reads once
+  // (32 rows of 2,048 pages, 8 heads of 128: 35 -> 20 us).
+  const int block = static_cast<int>(blockIdx.x), eights = a.num_tokens / 8 * 8 * a.kv_heads;
+  int h = block % a.kv_heads;
+  int64_t t = block / a.kv_heads;
+  if (block < eights) h = block / 8 % a.kv_heads, t = block / 8 / a.kv_heads * 8 + block % 8;
+  // q is asked for first: nothing of it waits for the request's row of the table
+  const int tiles = (a.group + 15) / 16;
+  const uint16_t* const q = a.q + t * a.q_tok_stride + static_cast<int64_t>(h) * a.group * a.q_head_stride;
+  const bool some = tid < a.group * (D / 8);
+  float v[8] = {};
+  if (some) load_q8(q + tid / (D / 8) * a.q_head_stride + 8 * (tid % (D / 8)), a.q_aligned, v);
+  const int64_t pos = a.positions[t];
   const int b = a.req_ids[t];
   if (b < 0 || b >= a.num_seqs) return;
   int32_t* const out = a.ids + t * a.ids_tok_stride + h * a.ids_head_stride;
-  const int64_t pos = a.positions[t];
-  const int all = pos < 0 ? 0 : static_cast<int>(min(pos / kPageTokens + 1, static_cast<int64_t>(a.bt_width)));
-  const int nb = min(all, a.max_blocks);
 
-  // q's codes
-  const int tiles = (a.group + 15) / 16;
+  // the wave's pages, asked for before anything waits
+  const int32_t* bt = a.block_table + b * a.bt_stride;
+  const int base = wave * KPT * 64;
+  auto page_of = [&](int c, int end) {
+    const int lp = base + 64 * c + lane;
+    return lp < end ? bt[lp] : -1;
+  };
+  int page[kAhead ? KPT : 1];
+  if constexpr (kAhead) {
+#pragma unroll
+    for (int c = 0; c < KPT; ++c) page[c] = page_of(c, min(a.max_blocks, a.bt_width));
+  }
+  const int all = pos < 0 ? 0 : static_cast<int>(min(pos / kPageTokens + 1, static_cast<int64_t>(a.bt_width)));
+  const int nb = __builtin_amdgcn_readfirstlane(min(all, a.max_blocks));
+  const int chunks = min(max((nb - base + 63) / 64, 0), KPT);  // of this wave
+
+  // q's codes: one exponent for the group; heads again where a tile has rows left
   float top = 0.0f;
-  for (int i = tid; i < a.group * D; i += kSelThreads) {
-    const int gh = i / D;
-    top = fmaxf(top, fabsf(bf16_to_f32(a.q[t * a.q_tok_stride + (h * a.group + gh) * a.q_head_stride + i % D])));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+  for (int i = tid + kThreads; i < a.group * (D / 8); i += kThreads) {
+    load_q8(q + i / (D / 8) * a.q_head_stride + 8 * (i % (D / 8)), a.q_aligned, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
   }
   top = wave_max_xor(top, 64);
   if (lane == 0) red[wave] = top;
+  for (int i = tid; i < kSelBins; i += kThreads) bins[i] = 0;
+  if (tid == 0) found[1] = 0xffffffffu;
   __syncthreads();
-  for (int w = 0; w < kSelWaves; ++w) top = fmaxf(top, red[w]);
-  const float qs = exp2i(pow2_exponent(top, kInv127));
-  for (int i = tid; i < tiles * 16 * D; i += kSelThreads) {
-    const int gh = (i / D) % a.group;  // heads again where a tile has rows left
-    const float x = bf16_to_f32(a.q[t * a.q_tok_stride + (h * a.group + gh) * a.q_head_stride + i % D]);
-    qc[i] = static_cast<int8_t>(fminf(fmaxf(rintf(x / qs), -127.0f), 127.0f));
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, red[w]);
+  const float qi = 1.0f / exp2i(pow2_exponent(top, kInv127));  // a power of two: products are exact
+  for (int i = tid; i < tiles * 16 * (D / 8); i += kThreads) {
+    const int row = i / (D / 8), at = 8 * (i % (D / 8));
+    load_q8(q + row % a.group * a.q_head_stride + at, a.q_aligned, v);
+    uint32_t w[2] = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int code = static_cast<int>(fminf(fmaxf(rintf(v[e] * qi), -127.0f), 127.0f));
+      w[e >> 2] |= static_cast<uint32_t>(code & 0xff) << (8 * (e & 3));
+    }
+    *reinterpret_cast<uint2*>(qc + row * kRow + at) = make_uint2(w[0], w[1]);
   }
   __syncthreads();
 
-  // keys: 64 pages a wave and round, as four tiles of 16
+  // keys: a chunk is four tiles of 16 pages; the mean keys of the next chunk
+  // are on their way while this one is multiplied
   const int m = lane & 15, g = lane >> 4;
-  const int32_t* bt = a.block_table + b * a.bt_stride;
-  for (int c = wave; c * 64 < nb; c += kSelWaves) {
-    const int lp = 64 * c + lane;
-    int64_t page = lp < nb ? bt[lp] : -1;
-    if (page >= a.num_pages) page = -1;
-    float scale = 0.0f;
-    if (page >= 0) scale = reinterpret_cast<const float*>(a.summary + page * a.summary_stride + a.kv_heads * D)[h];
-    i32x4 mk[4][S];
+  i32x4 qa[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) qa[s] = *reinterpret_cast<const i32x4*>(qc + m * kRow + 64 * s + 16 * g);
+  i32x4 mk[kBuf][4][S];
+  float scale[kBuf];
+  bool live[kBuf];
+  auto fetch = [&](int c, int buf) {
+    int pg = kAhead ? page[kAhead ? c : 0] : page_of(c, nb);
+    if (pg >= a.num_pages || base + 64 * c + lane >= nb) pg = -1;
+    live[buf] = pg >= 0;
+    scale[buf] = 0.0f;
+    if (pg >= 0) scale[buf] = reinterpret_cast<const float*>(a.summary + pg * a.summary_stride + a.kv_heads * D)[h];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t pg = __shfl(static_cast<int>(page), 16 * u + m, 64);
+      const int64_t p = __shfl(pg, 16 * u + m, 64);
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        mk[u][s] = i32x4{};
-        if (pg >= 0)
-          mk[u][s] = *reinterpret_cast<const i32x4*>(a.summary + pg * a.summary_stride + h * D + 64 * s + 16 * g);
+        mk[buf][u][s] = i32x4{};
+        if (p >= 0)
+          mk[buf][u][s] = *reinterpret_cast<const i32x4*>(a.summary + p * a.summary_stride + h * D + 64 * s + 16 * g);
       }
     }
-    int best = 0;
+  };
+  uint32_t key[KPT];
+  if (kBuf == 2 && chunks > 0) fetch(0, 0);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      int mx = -0x7fffffff;
-      for (int r = 0; r < tiles; ++r) {
-        i32x4 acc = {};
+  for (int c = 0; c < KPT; ++c) {
+    key[c] = 0;
+    if (c < chunks) {
+      if (kBuf == 1) fetch(c, 0);
+      else if (c + 1 < KPT && c + 1 < chunks) fetch(c + 1 < KPT ? c + 1 : 0, (c + 1) & 1);
+      const int buf = kBuf == 1 ? 0 : c & 1;
+      int best = 0;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const i32x4 qa = *reinterpret_cast<const i32x4*>(qc + (16 * r + m) * D + 64 * s + 16 * g);
-          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa, mk[u][s], acc, 0, 0, 0);
+      for (int u = 0; u < 4; ++u) {
+        int mx = -0x7fffffff;
+        for (int r = 0; r < tiles; ++r) {
+          i32x4 acc = {};
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            const i32x4 x = r ? *reinterpret_cast<const i32x4*>(qc + (16 * r + m) * kRow + 64 * s + 16 * g) : qa[s];
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, mk[buf][u][s], acc, 0, 0, 0);
+          }
+          mx = max(max(mx, max(acc[0], acc[1])), max(acc[2], acc[3]));
         }
-        mx = max(max(mx, max(acc[0], acc[1])), max(acc[2], acc[3]));
+        mx = max(mx, __shfl_xor(mx, 16, 64));
+        mx = max(mx, __shfl_xor(mx, 32, 64));
+        best = g == u ? mx : best;  // page 16 u + m of the chunk: this lane's
       }
-      mx = max(mx, __shfl_xor(mx, 16, 64));
-      mx = max(mx, __shfl_xor(mx, 32, 64));
-      if (g == u) best = mx;  // page 16 u + m of the chunk: this lane's
+      const int lp = base + 64 * c + lane;
+      const uint32_t k = lp < a.keep_first || lp >= all - a.keep_last ? 0xffffffffu
+                                                                      : score_key(static_cast<float>(best) * scale[buf]);
+      key[c] = live[buf] ? k : 0u;
     }
-    uint32_t key = 0;
-    if (page >= 0) {
-      key = score_key(static_cast<float>(best) * scale);
-      if (lp < a.keep_first || lp >= all - a.keep_last) key = 0xffffffffu;
-    }
-    keys[64 * c + lane] = key;
   }
-  const int chunks = (nb + 63) / 64;
 
-  // the n-th largest key: 11, 11 and 10 bits
-  uint32_t prefix = 0, mask = 0, need = static_cast<uint32_t>(a.n);
+  // The n-th largest key, 11, 11 and 10 bits: the keys above `thr` are taken, and
+  // the first `need` of those equal to it.  A bin whose keys are all needed ends
+  // the search, as the second round's mostly is.
+  uint32_t thr = 0, prefix = 0, mask = 0, need = static_cast<uint32_t>(a.n);
 #pragma unroll
   for (int round = 0; round < 3; ++round) {
     const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
     const uint32_t width = round == 2 ? 1024u : 2048u;
-    for (int i = tid; i < kSelBins; i += kSelThreads) bins[i] = 0;
-    if (tid == 0) found[0] = 0, found[1] = 0xffffffffu;
-    __syncthreads();
-    for (int i = tid; i < chunks * 64; i += kSelThreads) {
-      const uint32_t key = keys[i];
-      if ((key & mask) == prefix && key) atomicAdd(&bins[(key >> shift) & (width - 1)], 1u);
+#pragma unroll
+    for (int c = 0; c < KPT; ++c) {
+      if (c < chunks && key[c] && (key[c] & mask) == prefix) atomicAdd(&bins[(key[c] >> shift) & (width - 1)], 1u);
     }
     __syncthreads();
-    const uint32_t lo = bins[2 * tid], hi = bins[2 * tid + 1];
-    const uint32_t above = count_above(lo + hi, tmp);
-    // the bin with fewer than `need` keys above it and at least that many with its own
-    if (above < need && above + hi >= need) found[0] = 2 * tid + 1, found[1] = need - above;
-    else if (above + hi < need && above + hi + lo >= need) found[0] = 2 * tid, found[1] = need - above - hi;
-    __syncthreads();
-    if (found[1] == 0xffffffffu) {  // fewer keys than n: all of them
-      prefix = 1, mask = 0xffffffffu, need = 0;
-      break;
+    uint32_t own[kPer], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      own[i] = bins[kPer * tid + i];
+      mine += own[i];
     }
-    prefix |= found[0] << shift;
-    mask |= (width - 1) << shift;
-    need = found[1];
-    __syncthreads();
-  }
-  // keys above `prefix`, and the first `need` of those equal to it
-  for (int c = wave; c < chunks; c += kSelWaves) {
-    const uint32_t key = keys[64 * c + lane];
-    const uint64_t gt = __ballot(need ? key > prefix : key != 0), eq = __ballot(need && key == prefix);
-    if (lane == 0) chunk[c] = static_cast<uint32_t>(__builtin_popcountll(gt)) |
-                              static_cast<uint32_t>(__builtin_popcountll(eq)) << 16;
-  }
-  __syncthreads();
-  // sums of the chunks before each, in order; a wave's 64 chunks at a time
-  uint32_t gsum = 0, esum = 0;
-  if (tid < 512) {
-    const uint32_t v = tid < chunks ? chunk[tid] : 0;
-    gsum = v & 0xffffu, esum = v >> 16;
+    uint32_t up = mine;  // over the lanes from this one on
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) {
-      const uint32_t x = __shfl_up(gsum, k, 64), y = __shfl_up(esum, k, 64);
-      if (lane >= k) gsum += x, esum += y;
+      const uint32_t x = __shfl_down(up, k, 64);
+      if (lane + k < 64) up += x;
     }
-    if (lane == 63) bins[wave] = gsum, bins[16 + wave] = esum;
-    gsum -= v & 0xffffu, esum -= v >> 16;
+    if (lane == 0) sums[0][wave] = up;
+    __syncthreads();
+    uint32_t above = up - mine;  // keys in the bins above this thread's
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) above += w > wave ? sums[0][w] : 0u;
+    // the bin with fewer than `need` keys above it and at least that many with its own
+#pragma unroll
+    for (int i = kPer - 1; i >= 0; --i) {
+      bins[kPer * tid + i] = 0;  // for the next round
+      if (above < need && above + own[i] >= need) found[0] = kPer * tid + i, found[1] = need - above, found[2] = own[i];
+      above += own[i];
+    }
+    __syncthreads();
+    const uint32_t bin = found[0], left = found[1], held = found[2];
+    if (left == 0xffffffffu) {  // round 0, fewer keys than n: all of them
+      need = 0;
+      break;
+    }
+    prefix |= bin << shift;
+    mask |= (width - 1) << shift;
+    thr = prefix, need = left;
+    if (left == held) {
+      thr = prefix ? prefix - 1 : 0, need = 0;
+      break;
+    }
+  }
+
+  // in order
+  uint32_t gt_sum = 0, eq_sum = 0;
+#pragma unroll
+  for (int c = 0; c < KPT; ++c) {
+    if (c < chunks) {
+      gt_sum += static_cast<uint32_t>(__builtin_popcountll(__ballot(key[c] > thr)));
+      eq_sum += static_cast<uint32_t>(__builtin_popcountll(__ballot(need && key[c] == thr)));
+    }
   }
   __syncthreads();
-  uint32_t* const gb = bins + 64;
-  uint32_t* const eb = bins + 64 + 512;
-  if (tid < 512) {
-    for (int w = 0; w < wave; ++w) gsum += bins[w], esum += bins[16 + w];
-    gb[tid] = gsum, eb[tid] = esum;
-  }
+  if (lane == 0) sums[0][wave] = gt_sum, sums[1][wave] = eq_sum;
   __syncthreads();
-  uint32_t total = 0;
-  if (chunks) {
-    const uint32_t last = chunk[chunks - 1];
-    total = gb[chunks - 1] + (last & 0xffffu) + min(eb[chunks - 1] + (last >> 16), need);
+  uint32_t gb = 0, eb = 0, total = 0, equal = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w == wave) gb = total, eb = equal;
+    total += sums[0][w], equal += sums[1][w];
   }
-  for (int c = wave; c < chunks; c += kSelWaves) {
-    const uint32_t key = keys[64 * c + lane];
-    const bool is_gt = need ? key > prefix : key != 0, is_eq = need && key == prefix;
-    const uint64_t below = (1ull << lane) - 1;
-    const uint32_t gr = gb[c] + static_cast<uint32_t>(__builtin_popcountll(__ballot(is_gt) & below));
-    const uint32_t er = eb[c] + static_cast<uint32_t>(__builtin_popcountll(__ballot(is_eq) & below));
-    if (is_gt || (is_eq && er < need)) out[gr + min(er, need)] = 64 * c + lane;
+  total += min(equal, need);
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int c = 0; c < KPT; ++c) {
+    if (c < chunks) {
+      const bool is_gt = key[c] > thr, is_eq = need && key[c] == thr;
+      const uint64_t gt = __ballot(is_gt), eq = __ballot(is_eq);
+      const uint32_t gr = gb + static_cast<uint32_t>(__builtin_popcountll(gt & below));
+      const uint32_t er = eb + static_cast<uint32_t>(__builtin_popcountll(eq & below));
+      if (is_gt || (is_eq && er < need)) out[gr + min(er, need)] = base + 64 * c + lane;
+      gb += static_cast<uint32_t>(__builtin_popcountll(gt));
+      eb += static_cast<uint32_t>(__builtin_popcountll(eq));
+    }
   }
-  for (uint32_t i = total + tid; i < static_cast<uint32_t>(a.n); i += kSelThreads) out[i] = -1;
+  for (uint32_t i = total + tid; i < static_cast<uint32_t>(a.n); i += kThreads) out[i] = -1;
+}
+
+template <int D>
+static void launch_select(const GqaSelectArgs& a, int64_t grid, hipStream_t s) {
+  const dim3 g(static_cast<uint32_t>(grid));
+  if (a.max_blocks <= 2048 && grid >= 512) gqa_block_select_kernel<D, 4, 8><<<g, 256, 0, s>>>(a);
+  else if (a.max_blocks <= 2048) gqa_block_select_kernel<D, 16, 2><<<g, 1024, 0, s>>>(a);
+  else if (a.max_blocks <= 8192) gqa_block_select_kernel<D, 16, 8><<<g, 1024, 0, s>>>(a);
+  else gqa_block_select_kernel<D, 16, 32><<<g, 1024, 0, s>>>(a);
 }
 
 }  // namespace ekv
@@ -243,6 +315,7 @@ extern "C" int ekv_gqa_block_select(const uint16_t* q, int64_t q_tok_stride, int
   EKV_CHECK(grid < (int64_t{1} << 31), "too many rows for one call");
   GqaSelectArgs a{};
   a.q = q, a.q_tok_stride = q_tok_stride, a.q_head_stride = q_head_stride;
+  a.q_aligned = aligned16(q) && q_tok_stride % 8 == 0 && q_head_stride % 8 == 0;
   a.num_tokens = num_tokens, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
   a.summary = summary, a.summary_stride = summary_stride, a.num_pages = num_pages;
   a.block_table = block_table, a.bt_stride = bt_stride, a.bt_width = bt_width, a.num_seqs = num_seqs;
@@ -250,12 +323,9 @@ extern "C" int ekv_gqa_block_select(const uint16_t* q, int64_t q_tok_stride, int
   a.max_blocks = (max_len + kPageTokens - 1) / kPageTokens;
   a.n = num_blocks, a.keep_first = keep_first, a.keep_last = keep_last;
   a.ids = blocks, a.ids_tok_stride = blocks_tok_stride, a.ids_head_stride = blocks_head_stride;
-  const uint32_t lds = static_cast<uint32_t>((a.max_blocks + 63) / 64 * 64) * 4;
-  auto* const kernel = dim == 64 ? gqa_block_select_kernel<64>
-                       : dim == 128 ? gqa_block_select_kernel<128> : gqa_block_select_kernel<256>;
-  if (lds > 32768)  // over 64 KB with the static part
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(lds));
-  kernel<<<dim3(static_cast<uint32_t>(grid)), kSelThreads, lds, static_cast<hipStream_t>(stream)>>>(a);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dim == 64) launch_select<64>(a, grid, s);
+  else if (dim == 128) launch_select<128>(a, grid, s);
+  else launch_select<256>(a, grid, s);
   return ekv_launch_status();
 }

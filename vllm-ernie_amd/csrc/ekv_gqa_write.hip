@@ -126,17 +126,109 @@ struct GqaAppendArgs {
   RopeArgs rope;
 };
 
-__device__ __forceinline__ float fp8_value(uint32_t byte) {
-  return __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(byte), false)[0];
+// Lanes 32 .. 63 of x change places with lanes 0 .. 31 of y.
+__device__ __forceinline__ void swap32(uint32_t& x, uint32_t& y) {
+  const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  x = r[0], y = r[1];
 }
+// Lanes 16 .. 31 (48 .. 63) of x change places with lanes 0 .. 15 (32 .. 47) of y.
+__device__ __forceinline__ void swap16(uint32_t& x, uint32_t& y) {
+  const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+  x = r[0], y = r[1];
+}
+
+// A key row of L lanes with E pieces of 8 channels each: norm and rotation as
+// qk_norm_rope has them, sums and products in the same order.
+template <int L, int E>
+__device__ __forceinline__ void prep_key(float (&v)[E][8], const GqaAppendArgs& a, const float (&w)[E][8], int64_t pos,
+                                         int j) {
+  if (a.k_w) {
+    float s[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      s[e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[e] = __fmaf_rn(v[e][i], v[e][i], s[e]);
+#pragma unroll
+      for (int m = L >> 1; m > 0; m >>= 1) s[e] += __shfl_xor(s[e], m, 64);
+    }
+    const float sum = E == 2 ? s[0] + s[E - 1] : s[0];
+    const float r = 1.0f / sqrtf(sum / static_cast<float>(8 * L * E) + a.eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[e][i] = v[e][i] * r * w[e][i];
+    }
+  }
+  float c[E][8], s[E][8];
+#pragma unroll
+  for (int e = 0; e < E; ++e) rope_factors(a.rope, pos, E * j + e, c[e], s[e]);
+  if constexpr (E == 1) {
+    row_rope<L>(v[0], a.rope, j, c[0], s[0]);
+  } else if (a.rope.interleaved) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) row_rope<L>(v[e], a.rope, E * j + e, c[e], s[e]);
+  } else {  // the partner is a piece of this lane or another one
+    const int hop = a.rope.rope >> 4, lane = static_cast<int>(threadIdx.x) & 63;
+    float y[E][8];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int q = E * j + e, at = 8 * q - a.rope.offset;
+      const bool in = at >= 0 && at < a.rope.rope, low = at < (a.rope.rope >> 1);
+      const int from = in ? (low ? q + hop : q - hop) : q;
+      const int src = (lane & ~(L - 1)) + from / E;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p0 = __shfl(v[0][i], src, 64), p1 = __shfl(v[E - 1][i], src, 64);
+        const float p = from % E ? p1 : p0;
+        y[e][i] = low ? v[e][i] * c[e][i] - p * s[e][i] : v[e][i] * c[e][i] + p * s[e][i];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[e][i] = y[e][i];
+    }
+  }
+}
+
+// Four dwords of four bytes -> out[k] holds byte k of each.
+__device__ __forceinline__ void transpose4(const uint32_t (&a)[4], uint32_t (&out)[4]) {
+  const uint32_t l0 = __builtin_amdgcn_perm(a[1], a[0], 0x05010400u), h0 = __builtin_amdgcn_perm(a[1], a[0], 0x07030602u);
+  const uint32_t l1 = __builtin_amdgcn_perm(a[3], a[2], 0x05010400u), h1 = __builtin_amdgcn_perm(a[3], a[2], 0x07030602u);
+  out[0] = __builtin_amdgcn_perm(l1, l0, 0x05040100u), out[1] = __builtin_amdgcn_perm(l1, l0, 0x07060302u);
+  out[2] = __builtin_amdgcn_perm(h1, h0, 0x05040100u), out[3] = __builtin_amdgcn_perm(h1, h0, 0x07060302u);
+}
+
+__device__ __forceinline__ uint32_t fp8x4_codes(float a, float b, float c, float d) {
+  return f32x2_to_fp8(a, b) | f32x2_to_fp8(c, d) << 16;
+}
+
+// Codes times a power of two, coded again.
+__device__ __forceinline__ uint32_t fp8x4_scaled(uint32_t w, float r) {
+  const f32x4 x = fp8x4_to_f32(w) * r;
+  return fp8x4_codes(x[0], x[1], x[2], x[3]);
+}
+
+// Lane (i, j) of wave g holds 8 E channels of the tokens 16 t + 4 g + i, t = 0 ..
+// 3: V's 16 bytes of (channel, g) lie in the four lanes i of a wave, which hand
+// each other dwords by two swaps of half waves and half halves, and turn bytes
+// in registers.  No LDS holds rows or codes.
+template <int D>
+struct AppendShape {
+  static constexpr int kLanes = D == 64 ? 8 : 16;    // lanes of a row
+  static constexpr int kChunks = D == 256 ? 2 : 1;   // 8-channel pieces of a lane
+  static constexpr int kThreads = D == 64 ? 128 : 256;
+};
 
 template <int D>
 __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
-  constexpr int LPR = D / 8, RPP = 256 / LPR, PASSES = kPageTokens / RPP;  // lanes a row, rows a pass
-  __shared__ __attribute__((aligned(16))) uint8_t tile[kPageTokens * (D + 16)];
-  __shared__ float red[2][4];
-  __shared__ float sums[4][D];
-  const int tid = static_cast<int>(threadIdx.x), wave = tid >> 6, j = tid & (LPR - 1), r0 = tid / LPR;
+  constexpr int L = AppendShape<D>::kLanes, E = AppendShape<D>::kChunks, kWaves = AppendShape<D>::kThreads / 64;
+  __shared__ float red[2][kWaves];
+  __shared__ float sums[kWaves * (D == 64 ? 2 : 1)][D];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & (L - 1), i = lane >> 4, g = D == 64 ? 2 * wave + ((lane >> 3) & 1) : wave;
   const int h = block % a.kv_heads;
   const int slot = block / a.kv_heads % a.page_slots, b = block / a.kv_heads / a.page_slots;
   const int t0 = a.qsl[b], n = min(a.qsl[b + 1], a.num_tokens) - t0;
@@ -148,137 +240,191 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
   const int end = static_cast<int>(min(p0 + n - base, static_cast<int64_t>(kPageTokens)));  // rows first .. end - 1
   if (end <= first || lp >= a.bt_width) return;
   const int64_t page = a.block_table[b * a.bt_stride + lp];
-  if (page < 0 || page >= a.num_pages) return;
   const int64_t tok = t0 + base - p0;  // token of the page's row 0
 
+  // the new rows, asked for beside the page's place
+  float kx[4][E][8], vx[4][E][8];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int r = 16 * t + 4 * g + i;
+    const bool have = r >= first && r < end;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = 8 * (E * j + e);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) kx[t][e][x] = vx[t][e][x] = 0.0f;
+      if (have) {
+        load_row8(a.k + (tok + r) * a.k_tok_stride + h * a.k_head_stride + c, a.k_aligned, kx[t][e]);
+        load_row8(a.v + (tok + r) * a.v_tok_stride + h * a.v_head_stride + c, a.v_aligned, vx[t][e]);
+      }
+    }
+  }
+  const bool live = page >= 0 && page < a.num_pages;
   uint8_t* const pg = a.cache + page * a.page_stride;
   uint8_t* const kp = pg + static_cast<int64_t>(h) * kPageTokens * D;
   uint8_t* const vp = pg + static_cast<int64_t>(a.kv_heads + h) * kPageTokens * D;
   float* const ks = reinterpret_cast<float*>(pg + 2ll * a.kv_heads * kPageTokens * D) + h;
   float* const vs = ks + a.kv_heads;
+  float kold = 0.0f, vold = 0.0f;
+  if (live && first) kold = *ks, vold = *vs;
 
-  // the new rows, and their largest values
-  float kx[PASSES][8], vx[PASSES][8], kmax = 0.0f, vmax = 0.0f;
-  float w[8];
-  if (a.prep && a.k_w) load_weight8(a.k_w, a.k_w_bf16, j, w);
+  if (a.prep) {
+    float w[E][8];
+    if (a.k_w) {
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = i * RPP + r0;
-    const bool have = r >= first && r < end;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) kx[i][e] = 0.0f, vx[i][e] = 0.0f;
-    if (have) {
-      load_row8(a.k + (tok + r) * a.k_tok_stride + h * a.k_head_stride + 8 * j, a.k_aligned, kx[i]);
-      load_row8(a.v + (tok + r) * a.v_tok_stride + h * a.v_head_stride + 8 * j, a.v_aligned, vx[i]);
-    }
-    if (a.prep) {
-      float c[8], s[8];
-      rope_factors(a.rope, have ? base + r : -1, j, c, s);
-      if (a.k_w) row_rms_norm<LPR>(kx[i], w, D, a.eps);
-      row_rope<LPR>(kx[i], a.rope, j, c, s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) kx[i][e] = have ? bf16_to_f32(f32_to_bf16(kx[i][e])) : 0.0f;
+      for (int e = 0; e < E; ++e) load_weight8(a.k_w, a.k_w_bf16, E * j + e, w[e]);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) kmax = fmaxf(kmax, fabsf(kx[i][e])), vmax = fmaxf(vmax, fabsf(vx[i][e]));
+    for (int t = 0; t < 4; ++t) {
+      const int r = 16 * t + 4 * g + i;
+      const bool have = r >= first && r < end;
+      prep_key<L, E>(kx[t], a, w, have ? base + r : -1, j);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) kx[t][e][x] = have ? bf16_to_f32(f32_to_bf16(kx[t][e][x])) : 0.0f;
+      }
+    }
+  }
+  float kmax = 0.0f, vmax = 0.0f;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) kmax = fmaxf(kmax, fabsf(kx[t][e][x])), vmax = fmaxf(vmax, fabsf(vx[t][e][x]));
+    }
   }
   kmax = wave_max_xor(kmax, 64);
   vmax = wave_max_xor(vmax, 64);
-  if ((tid & 63) == 0) red[0][wave] = kmax, red[1][wave] = vmax;
+  if (lane == 0) red[0][wave] = kmax, red[1][wave] = vmax;
   __syncthreads();
-  kmax = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  vmax = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
-  const float kold = first ? *ks : 0.0f, vold = first ? *vs : 0.0f;
+  if (!live) return;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) kmax = fmaxf(kmax, red[0][w]), vmax = fmaxf(vmax, red[1][w]);
   const float knew = fmaxf(exp2i(pow2_exponent(kmax, kInv448)), kold);
   const float vnew = fmaxf(exp2i(pow2_exponent(vmax, kInv448)), vold);
   const bool kgrow = first && knew > kold, vgrow = first && vnew > vold;
   const float ki = 1.0f / knew, vi = 1.0f / vnew;  // powers of two: the products below are exact
   const float kr = kold * ki, vr = vold * vi;
 
-  // K codes of the new rows; V codes to LDS, row by row
+  // K: rows as they are; earlier ones again in the larger scale.  For the
+  // summary kx becomes the stored values in code units.
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = i * RPP + r0;
-    if (r >= first && r < end) {
-      uint2 kc, vc;
-      kc.x = f32x2_to_fp8(kx[i][0] * ki, kx[i][1] * ki) | f32x2_to_fp8(kx[i][2] * ki, kx[i][3] * ki) << 16;
-      kc.y = f32x2_to_fp8(kx[i][4] * ki, kx[i][5] * ki) | f32x2_to_fp8(kx[i][6] * ki, kx[i][7] * ki) << 16;
-      vc.x = f32x2_to_fp8(vx[i][0] * vi, vx[i][1] * vi) | f32x2_to_fp8(vx[i][2] * vi, vx[i][3] * vi) << 16;
-      vc.y = f32x2_to_fp8(vx[i][4] * vi, vx[i][5] * vi) | f32x2_to_fp8(vx[i][6] * vi, vx[i][7] * vi) << 16;
-      *reinterpret_cast<uint2*>(kp + r * D + 8 * j) = kc;
-      *reinterpret_cast<uint2*>(tile + r * (D + 16) + 8 * j) = vc;
-    } else if (r < first && (kgrow || a.summary)) {
-      // earlier rows: again in the larger scale
-      uint2 kc = *reinterpret_cast<const uint2*>(kp + r * D + 8 * j);
-      if (kgrow) {
-        const f32x4 lo = fp8x4_to_f32(kc.x) * kr, hi = fp8x4_to_f32(kc.y) * kr;
-        kc.x = f32x2_to_fp8(lo[0], lo[1]) | f32x2_to_fp8(lo[2], lo[3]) << 16;
-        kc.y = f32x2_to_fp8(hi[0], hi[1]) | f32x2_to_fp8(hi[2], hi[3]) << 16;
-        *reinterpret_cast<uint2*>(kp + r * D + 8 * j) = kc;
+  for (int t = 0; t < 4; ++t) {
+    const int r = 16 * t + 4 * g + i;
+    uint8_t* const dst = kp + r * D + 8 * E * j;
+    uint32_t kc[2 * E] = {};
+    const bool have = r >= first && r < end, old = r < first && (kgrow || a.summary);
+    if (have) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float(&x)[8] = kx[t][e];
+        kc[2 * e] = fp8x4_codes(x[0] * ki, x[1] * ki, x[2] * ki, x[3] * ki);
+        kc[2 * e + 1] = fp8x4_codes(x[4] * ki, x[5] * ki, x[6] * ki, x[7] * ki);
       }
-      if (a.summary) {
-        const f32x4 lo = fp8x4_to_f32(kc.x), hi = fp8x4_to_f32(kc.y);
+    } else if (old) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) kx[i][e] = lo[e] * knew, kx[i][4 + e] = hi[e] * knew;
+      for (int e = 0; e < 2 * E; ++e) {
+        kc[e] = reinterpret_cast<const uint32_t*>(dst)[e];
+        if (kgrow) kc[e] = fp8x4_scaled(kc[e], kr);
+      }
+    }
+    if (have || (old && kgrow)) {
+      if constexpr (E == 2) *reinterpret_cast<uint4*>(dst) = make_uint4(kc[0], kc[1], kc[2], kc[3]);
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(kc[0], kc[1]);
+    }
+    if (a.summary) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const f32x4 lo = fp8x4_to_f32(kc[2 * e]), hi = fp8x4_to_f32(kc[2 * e + 1]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) kx[t][e][x] = lo[x], kx[t][e][4 + x] = hi[x];
       }
     }
   }
-  __syncthreads();
 
-  // V by channel: 16 bytes at a time, old tokens' bytes requantized, those behind the last row kept
-  for (int u = tid; u < 4 * D; u += 256) {
-    const int c = u >> 2, g = u & 3;
-    uint8_t* const dst = vp + c * kPageTokens + 16 * g;
-    const bool whole = first == 0 && end == kPageTokens;
-    uint32_t out[4] = {};
-    if (!whole) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(dst);
+  // V: this lane ends with 4 channels (half of its pieces: i & 1) of the tokens
+  // 16 t + 4 g + 0 .. 3 of two t (2 (i >> 1), + 1)
+  uint32_t fresh[2], older[2], any = 0;  // bytes of its tokens that are new, or before them
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    fresh[u] = older[u] = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int r = 16 * (2 * (i >> 1) + u) + 4 * g + x;
+      fresh[u] |= (r >= first) & (r < end) ? 0xffu << (8 * x) : 0u;
+      older[u] |= r < first ? 0xffu << (8 * x) : 0u;
+    }
+    any |= fresh[u] | (vgrow ? older[u] : 0u);
+  }
+  const bool all_new = (fresh[0] & fresh[1]) == 0xffffffffu;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    uint32_t x[4][2];  // [t][half]: four channels of this lane's token
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      uint32_t word = out[t];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * t + 4 * g + i;
-        uint32_t byte = (word >> (8 * i)) & 0xffu;
-        if (r >= first && r < end) byte = tile[r * (D + 16) + c];
-        else if (r < first && vgrow) byte = f32x2_to_fp8(fp8_value(byte) * vr, 0.0f) & 0xffu;
-        word = (word & ~(0xffu << (8 * i))) | byte << (8 * i);
-      }
-      out[t] = word;
+      const float(&y)[8] = vx[t][e];
+      x[t][0] = fp8x4_codes(y[0] * vi, y[1] * vi, y[2] * vi, y[3] * vi);
+      x[t][1] = fp8x4_codes(y[4] * vi, y[5] * vi, y[6] * vi, y[7] * vi);
     }
-    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(out);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {  // lower lanes: t = s from both halves of the wave; upper lanes: t = s + 2
+#pragma unroll
+      for (int half = 0; half < 2; ++half) swap32(x[s][half], x[s + 2][half]);
+    }
+    uint32_t y[2][4];  // [t][lane i]
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {  // even 16 lanes: half 0 from both, odd ones: half 1
+        swap16(x[s + 2 * k][0], x[s + 2 * k][1]);
+        y[s][2 * k] = x[s + 2 * k][0], y[s][2 * k + 1] = x[s + 2 * k][1];
+      }
+    }
+    uint32_t z[2][4];
+    transpose4(y[0], z[0]);
+    transpose4(y[1], z[1]);
+    uint8_t* const dst = vp + (8 * (E * j + e) + 4 * (i & 1)) * kPageTokens + 16 * g + 8 * (i >> 1);
+    if (any) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint2 out = make_uint2(z[0][c], z[1][c]);
+        if (!all_new) {
+          uint2 was = *reinterpret_cast<const uint2*>(dst + c * kPageTokens);
+          if (vgrow) {
+            was.x = (was.x & ~older[0]) | (fp8x4_scaled(was.x, vr) & older[0]);
+            was.y = (was.y & ~older[1]) | (fp8x4_scaled(was.y, vr) & older[1]);
+          }
+          out.x = (out.x & fresh[0]) | (was.x & ~fresh[0]);
+          out.y = (out.y & fresh[1]) | (was.y & ~fresh[1]);
+        }
+        *reinterpret_cast<uint2*>(dst + c * kPageTokens) = out;
+      }
+    }
   }
   if (tid == 0) *ks = knew, *vs = vnew;
 
   if (a.summary) {  // uniform over the workgroup
     // Sums of codes: multiples of 2^-9 below 2^15, exact in fp32 in any order.
-    float sum[8] = {};
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int r = i * RPP + r0;
-      if (r < end) {
+    for (int e = 0; e < E; ++e) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = kx[i][e] * ki;
-          sum[e] += r < first ? y : fp8_value(f32x2_to_fp8(y, 0.0f) & 0xffu);
-        }
+      for (int x = 0; x < 8; ++x) {
+        float s = (kx[0][e][x] + kx[1][e][x]) + (kx[2][e][x] + kx[3][e][x]);
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (i == 0) sums[g][8 * (E * j + e) + x] = s;
       }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-#pragma unroll
-      for (int m = LPR; m < 64; m <<= 1) sum[e] += __shfl_xor(sum[e], m, 64);
-    }
-    if ((tid & 63) < LPR) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sums[wave][8 * j + e] = sum[e];
     }
     __syncthreads();
     float mean = 0.0f;
-    if (tid < D) mean = (((sums[0][tid] + sums[1][tid]) + sums[2][tid]) + sums[3][tid]) / static_cast<float>(end);
+    if (tid < D) mean = ((sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid])) / static_cast<float>(end);
     float top = wave_max_xor(fabsf(mean), 64);
-    if ((tid & 63) == 0) red[0][wave] = top;
+    if (lane == 0) red[0][wave] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red[0][w]);
     const float s = exp2i(pow2_exponent(top, kInv127));
     uint8_t* const rec = a.summary + page * a.summary_stride;
     if (tid < D) {
@@ -290,19 +436,20 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(256) gqa_append_kernel(GqaAppendArgs a) {
+__global__ void __launch_bounds__(AppendShape<D>::kThreads) gqa_append_kernel(GqaAppendArgs a) {
   gqa_append_block<D>(a, static_cast<int>(blockIdx.x));
 }
 
 // The append's workgroups first, then those of q's norm and rotation.
 template <int D>
-__global__ void __launch_bounds__(256) gqa_prologue_kernel(GqaAppendArgs a, NormArgs q, int append_blocks) {
+__global__ void __launch_bounds__(AppendShape<D>::kThreads) gqa_prologue_kernel(GqaAppendArgs a, NormArgs q, int append_blocks) {
   const int block = static_cast<int>(blockIdx.x);
   if (block < append_blocks) {
     gqa_append_block<D>(a, block);
   } else {
     const int64_t units = norm_units(q, 0);
-    norm_unit<D / 8>(q, static_cast<int64_t>(block - append_blocks) * (2048 / D) + threadIdx.x / (D / 8), units, units);
+    constexpr int kRows = AppendShape<D>::kThreads * 8 / D;
+    norm_unit<D / 8>(q, static_cast<int64_t>(block - append_blocks) * kRows + threadIdx.x / (D / 8), units, units);
   }
 }
 
@@ -335,24 +482,24 @@ static int pow2_lanes(int dim) {
   return l;
 }
 
-static int launch_append(const GqaAppendArgs& a, const NormArgs* q, int dim, void* stream) {
+template <int D>
+static int launch_append_dim(const GqaAppendArgs& a, const NormArgs* q, hipStream_t s) {
+  constexpr int kThreads = AppendShape<D>::kThreads, kRows = kThreads * 8 / D;
   const int64_t append = static_cast<int64_t>(a.num_seqs) * a.page_slots * a.kv_heads;
-  int64_t blocks = append;
-  if (q) blocks += (norm_units(*q, 0) + 2048 / dim - 1) / (2048 / dim);
+  const int64_t blocks = append + (q ? (norm_units(*q, 0) + kRows - 1) / kRows : 0);
   EKV_CHECK(blocks < (int64_t{1} << 31), "too many rows for one call");
   if (!blocks) return kOk;
   const dim3 grid(static_cast<uint32_t>(blocks));
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (q) {
-    if (dim == 64) gqa_prologue_kernel<64><<<grid, 256, 0, s>>>(a, *q, static_cast<int>(append));
-    else if (dim == 128) gqa_prologue_kernel<128><<<grid, 256, 0, s>>>(a, *q, static_cast<int>(append));
-    else gqa_prologue_kernel<256><<<grid, 256, 0, s>>>(a, *q, static_cast<int>(append));
-  } else {
-    if (dim == 64) gqa_append_kernel<64><<<grid, 256, 0, s>>>(a);
-    else if (dim == 128) gqa_append_kernel<128><<<grid, 256, 0, s>>>(a);
-    else gqa_append_kernel<256><<<grid, 256, 0, s>>>(a);
-  }
+  if (q) gqa_prologue_kernel<D><<<grid, kThreads, 0, s>>>(a, *q, static_cast<int>(append));
+  else gqa_append_kernel<D><<<grid, kThreads, 0, s>>>(a);
   return ekv_launch_status();
+}
+
+static int launch_append(const GqaAppendArgs& a, const NormArgs* q, int dim, void* stream) {
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dim == 64) return launch_append_dim<64>(a, q, s);
+  if (dim == 128) return launch_append_dim<128>(a, q, s);
+  return launch_append_dim<256>(a, q, s);
 }
 
 // Checks and fills what the append and the prologue share; empty calls leave num_seqs 0.

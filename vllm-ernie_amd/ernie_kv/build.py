@@ -53,7 +53,7 @@ SOURCES = {
     "ekv_pages.hip": EXACT,
     "ekv_gqa_write.hip": EXACT,
     "ekv_gqa_attn.hip": MFMA_VGPR,
-    "ekv_gqa_select.hip": EXACT,
+    "ekv_gqa_select.hip": EXACT + MFMA_VGPR,
 }
 
 
