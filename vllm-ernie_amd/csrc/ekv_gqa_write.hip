@@ -47,6 +47,22 @@ __device__ __forceinline__ void load_row8(const uint16_t* p, bool aligned, float
   }
 }
 
+__device__ __forceinline__ uint4 load_raw8(const uint16_t* p, bool aligned) {
+  if (aligned) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = p[2 * i] | static_cast<uint32_t>(p[2 * i + 1]) << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ float row_max8(uint4 w, float top) {
+  float v[8];
+  unpack_bf16x8(w, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+  return top;
+}
+
 __device__ __forceinline__ void load_weight8(const void* w, int is_bf16, int j, float (&v)[8]) {
   if (is_bf16) {
 #pragma unroll
@@ -213,7 +229,8 @@ __device__ __forceinline__ uint32_t fp8x4_scaled(uint32_t w, float r) {
 // Lane (i, j) of wave g holds 8 E channels of the tokens 16 t + 4 g + i, t = 0 ..
 // 3: V's 16 bytes of (channel, g) lie in the four lanes i of a wave, which hand
 // each other dwords by two swaps of half waves and half halves, and turn bytes
-// in registers.  No LDS holds rows or codes.
+// in registers; a whole page's bytes pass through LDS once more, so that they
+// leave as whole lines.
 template <int D>
 struct AppendShape {
   static constexpr int kLanes = D == 64 ? 8 : 16;    // lanes of a row
@@ -225,7 +242,8 @@ template <int D>
 __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
   constexpr int L = AppendShape<D>::kLanes, E = AppendShape<D>::kChunks, kWaves = AppendShape<D>::kThreads / 64;
   __shared__ float red[2][kWaves];
-  __shared__ float sums[kWaves * (D == 64 ? 2 : 1)][D];
+  __shared__ float sums[4][D];
+  __shared__ __attribute__((aligned(16))) uint8_t tile[D * kPageTokens];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane & (L - 1), i = lane >> 4, g = D == 64 ? 2 * wave + ((lane >> 3) & 1) : wave;
@@ -242,8 +260,8 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
   const int64_t page = a.block_table[b * a.bt_stride + lp];
   const int64_t tok = t0 + base - p0;  // token of the page's row 0
 
-  // the new rows, asked for beside the page's place
-  float kx[4][E][8], vx[4][E][8];
+  // the new rows, asked for beside the page's place; they stay packed
+  uint4 kx[4][E], vx[4][E];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const int r = 16 * t + 4 * g + i;
@@ -251,11 +269,10 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = 8 * (E * j + e);
-#pragma unroll
-      for (int x = 0; x < 8; ++x) kx[t][e][x] = vx[t][e][x] = 0.0f;
+      kx[t][e] = vx[t][e] = make_uint4(0, 0, 0, 0);
       if (have) {
-        load_row8(a.k + (tok + r) * a.k_tok_stride + h * a.k_head_stride + c, a.k_aligned, kx[t][e]);
-        load_row8(a.v + (tok + r) * a.v_tok_stride + h * a.v_head_stride + c, a.v_aligned, vx[t][e]);
+        kx[t][e] = load_raw8(a.k + (tok + r) * a.k_tok_stride + h * a.k_head_stride + c, a.k_aligned);
+        vx[t][e] = load_raw8(a.v + (tok + r) * a.v_tok_stride + h * a.v_head_stride + c, a.v_aligned);
       }
     }
   }
@@ -278,11 +295,15 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
     for (int t = 0; t < 4; ++t) {
       const int r = 16 * t + 4 * g + i;
       const bool have = r >= first && r < end;
-      prep_key<L, E>(kx[t], a, w, have ? base + r : -1, j);
+      float v[E][8];
+#pragma unroll
+      for (int e = 0; e < E; ++e) unpack_bf16x8(kx[t][e], v[e]);
+      prep_key<L, E>(v, a, w, have ? base + r : -1, j);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
 #pragma unroll
-        for (int x = 0; x < 8; ++x) kx[t][e][x] = have ? bf16_to_f32(f32_to_bf16(kx[t][e][x])) : 0.0f;
+        for (int x = 0; x < 8; ++x) v[e][x] = have ? bf16_to_f32(f32_to_bf16(v[e][x])) : 0.0f;
+        kx[t][e] = pack_bf16x8(v[e]);
       }
     }
   }
@@ -290,10 +311,7 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-#pragma unroll
-      for (int x = 0; x < 8; ++x) kmax = fmaxf(kmax, fabsf(kx[t][e][x])), vmax = fmaxf(vmax, fabsf(vx[t][e][x]));
-    }
+    for (int e = 0; e < E; ++e) kmax = row_max8(kx[t][e], kmax), vmax = row_max8(vx[t][e], vmax);
   }
   kmax = wave_max_xor(kmax, 64);
   vmax = wave_max_xor(vmax, 64);
@@ -308,8 +326,10 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
   const float ki = 1.0f / knew, vi = 1.0f / vnew;  // powers of two: the products below are exact
   const float kr = kold * ki, vr = vold * vi;
 
-  // K: rows as they are; earlier ones again in the larger scale.  For the
-  // summary kx becomes the stored values in code units.
+  // K: rows as they are; earlier ones again in the larger scale.  sum: of the
+  // stored codes' values over this lane's tokens, exact in fp32 in any order
+  // (multiples of 2^-9 below 2^15).
+  float sum[E][8] = {};
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const int r = 16 * t + 4 * g + i;
@@ -319,7 +339,8 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
     if (have) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float(&x)[8] = kx[t][e];
+        float x[8];
+        unpack_bf16x8(kx[t][e], x);
         kc[2 * e] = fp8x4_codes(x[0] * ki, x[1] * ki, x[2] * ki, x[3] * ki);
         kc[2 * e + 1] = fp8x4_codes(x[4] * ki, x[5] * ki, x[6] * ki, x[7] * ki);
       }
@@ -339,7 +360,7 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
       for (int e = 0; e < E; ++e) {
         const f32x4 lo = fp8x4_to_f32(kc[2 * e]), hi = fp8x4_to_f32(kc[2 * e + 1]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) kx[t][e][x] = lo[x], kx[t][e][4 + x] = hi[x];
+        for (int x = 0; x < 4; ++x) sum[e][x] += lo[x], sum[e][4 + x] += hi[x];
       }
     }
   }
@@ -359,12 +380,14 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
     any |= fresh[u] | (vgrow ? older[u] : 0u);
   }
   const bool all_new = (fresh[0] & fresh[1]) == 0xffffffffu;
+  const bool whole = first == 0 && end == kPageTokens;  // uniform
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     uint32_t x[4][2];  // [t][half]: four channels of this lane's token
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const float(&y)[8] = vx[t][e];
+      float y[8];
+      unpack_bf16x8(vx[t][e], y);
       x[t][0] = fp8x4_codes(y[0] * vi, y[1] * vi, y[2] * vi, y[3] * vi);
       x[t][1] = fp8x4_codes(y[4] * vi, y[5] * vi, y[6] * vi, y[7] * vi);
     }
@@ -385,8 +408,15 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
     uint32_t z[2][4];
     transpose4(y[0], z[0]);
     transpose4(y[1], z[1]);
-    uint8_t* const dst = vp + (8 * (E * j + e) + 4 * (i & 1)) * kPageTokens + 16 * g + 8 * (i >> 1);
-    if (any) {
+    const int c0 = 8 * (E * j + e) + 4 * (i & 1), piece = 2 * g + (i >> 1);  // 8 bytes of a channel's 64
+    uint8_t* const dst = vp + c0 * kPageTokens + 8 * piece;
+    if (whole) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int at = piece ^ ((c0 >> 3) & 7);  // channels 8 apart share banks
+        *reinterpret_cast<uint2*>(tile + (c0 + c) * kPageTokens + 8 * at) = make_uint2(z[0][c], z[1][c]);
+      }
+    } else if (any) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint2 out = make_uint2(z[0][c], z[1][c]);
@@ -403,15 +433,22 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
       }
     }
   }
+  if (whole) {  // a channel's 64 bytes at a time
+    __syncthreads();
+    for (int u = tid; u < 4 * D; u += AppendShape<D>::kThreads) {
+      const int c = u >> 2, s = (c >> 3) & 7;
+      const uint4 w = *reinterpret_cast<const uint4*>(tile + c * kPageTokens + 16 * ((u & 3) ^ (s >> 1)));
+      *reinterpret_cast<uint4*>(vp + 16 * u) = s & 1 ? make_uint4(w.z, w.w, w.x, w.y) : w;
+    }
+  }
   if (tid == 0) *ks = knew, *vs = vnew;
 
   if (a.summary) {  // uniform over the workgroup
-    // Sums of codes: multiples of 2^-9 below 2^15, exact in fp32 in any order.
 #pragma unroll
     for (int e = 0; e < E; ++e) {
 #pragma unroll
       for (int x = 0; x < 8; ++x) {
-        float s = (kx[0][e][x] + kx[1][e][x]) + (kx[2][e][x] + kx[3][e][x]);
+        float s = sum[e][x];
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
         if (i == 0) sums[g][8 * (E * j + e) + x] = s;
