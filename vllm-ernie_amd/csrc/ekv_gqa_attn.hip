@@ -43,10 +43,63 @@ struct GqaAttnArgs {
   float* lse;
   int64_t lse_stride;
   // plan
-  int32_t tiles, units, splits, split_pages;
-  float* ws_o;              // [splits, T, heads, D]
-  float2* ws_ml;            // [splits, T, heads]: (reference in log2 units, sum)
+  int32_t tiles, units, splits, split_pages;  // units: (sequence, kv head, tile)
+  int32_t budget;           // 0, or the parts of a (kv head, tile) that its sequences share
+  int32_t slots, part_step; // workgroups, and how far apart those of a unit are
+  int2* ws_rows;            // [T, heads]: first workgroup, parts | row of its tile << 8
+  float2* ws_ml;            // [slots, rows]: (reference in log2 units, sum)
+  float* ws_o;              // [slots, rows, D]
 };
+
+// A workgroup's part of a unit.
+struct GqaPart {
+  int seq, h, tile;
+  int part, parts, first;   // first: the workgroup of part 0
+  int pages;                // of a part (static), or of the unit as far as known (dynamic)
+};
+
+// Which part of what workgroup i takes where up to 64 sequences share the chip
+// by their lengths: every workgroup finds the same smallest Q at which parts of
+// Q pages fit the budget.  A sequence's length is taken from its last row, which
+// decides the shares only.
+__device__ __forceinline__ bool find_part(const GqaAttnArgs& a, int i, GqaPart& p) {
+  const int lane = static_cast<int>(threadIdx.x) & 63, per = a.kv_heads * a.tiles;
+  int w = 0;
+  if (lane < a.num_seqs) {
+    const int t0 = a.qsl[lane], t1 = min(a.qsl[lane + 1], a.num_tokens);
+    if (t0 >= 0 && t1 > t0) {
+      const int64_t pos = a.positions[t1 - 1];
+      w = static_cast<int>(min(max(pos, static_cast<int64_t>(0)) / kPageTokens + 1, static_cast<int64_t>(max(a.bt_width, 1))));
+      if (a.window) w = min(w, a.split_pages);  // the most pages a tile sees
+    }
+  }
+  auto sum = [](int v) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
+    return __builtin_amdgcn_readfirstlane(v);
+  };
+  int q = max((sum(w) + a.budget - 1) / a.budget, 4), mine;
+  while (true) {
+    mine = w ? min(max(static_cast<int>(ceilf(static_cast<float>(w) * (1.0f / static_cast<float>(q)))), 1), 64) : 0;
+    if (sum(mine) <= a.budget) break;  // reached: from the longest sequence on there is one part each
+    q += (q >> 4) + 1;
+  }
+  int upto = mine;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int x = __shfl_up(upto, m, 64);
+    if (lane >= m) upto += x;
+  }
+  const int j = i / per, ht = i - j * per;
+  const uint64_t at = __ballot(j < upto && j >= upto - mine);
+  if (!at) return false;
+  p.seq = __builtin_ctzll(at);
+  p.h = ht % a.kv_heads, p.tile = ht / a.kv_heads;
+  p.parts = __builtin_amdgcn_readlane(mine, p.seq);
+  const int before = __builtin_amdgcn_readlane(upto, p.seq) - p.parts;
+  p.part = j - before, p.first = before * per + ht, p.pages = __builtin_amdgcn_readlane(w, p.seq);
+  return true;
+}
 
 // 8 e4m3fn codes times a power of two -> bf16.
 __device__ __forceinline__ bf16x8 fp8x8_to_bf16(uint32_t lo, uint32_t hi, float s) {
@@ -261,8 +314,16 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
   __shared__ float2 sml[4][16];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int unit = static_cast<int>(blockIdx.x) % a.units, split = static_cast<int>(blockIdx.x) / a.units;
-  const int h = unit % a.kv_heads, tile = unit / a.kv_heads % a.tiles, seq = unit / a.kv_heads / a.tiles;
+  GqaPart p;
+  const bool dynamic = !LIST && a.budget;
+  if (dynamic) {
+    if (!find_part(a, static_cast<int>(blockIdx.x), p)) return;
+  } else {
+    const int unit = static_cast<int>(blockIdx.x) % a.units;
+    p.h = unit % a.kv_heads, p.tile = unit / a.kv_heads % a.tiles, p.seq = unit / a.kv_heads / a.tiles;
+    p.part = static_cast<int>(blockIdx.x) / a.units, p.parts = a.splits, p.first = unit, p.pages = a.split_pages;
+  }
+  const int h = p.h, seq = p.seq;
 
   // the rows: (token, head of the group), flattened
   int t0, rows, b;
@@ -274,7 +335,7 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
     rows = (min(a.qsl[b + 1], a.num_tokens) - t0) * a.group;
     if (t0 < 0) return;
   }
-  const int r0 = tile * 16 * NT;
+  const int r0 = p.tile * 16 * NT;
   if (r0 >= rows) return;
 
   // lane i: the wave's i-th page of 64, its logical index and its place (-1:
@@ -288,8 +349,9 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
     return lp;
   };
   const bool early = LIST || !a.window;
-  int pb = split * a.split_pages, pe = LIST ? a.n_ids : a.bt_width;
-  if (split < a.splits - 1) pe = min(pe, pb + a.split_pages);
+  int share = dynamic ? (p.pages + p.parts - 1) / p.parts : p.pages;
+  int pb = p.part * share, pe = LIST ? a.n_ids : dynamic ? p.pages : a.bt_width;
+  if (p.part < p.parts - 1) pe = min(pe, pb + share);
   int page, lp;
   if (early) lp = list(pb + wave + 4 * lane, pe, page);
 
@@ -312,10 +374,15 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
   if constexpr (kQLds) __syncthreads();
   const int pmax = rr.pmax;
   const int low = a.window && pmax >= 0 ? max(rr.pmin - a.window + 1, 0) : 0;  // first token any row sees
+  bool listed = early;
   if (!LIST) {
-    const int last = pmax < 0 ? 0 : min(pmax / kPageTokens + 1, a.bt_width);
-    pb += low / kPageTokens;
-    pe = split == a.splits - 1 ? last : min(pb + a.split_pages, last);
+    const int last = pmax < 0 ? 0 : min(pmax / kPageTokens + 1, a.bt_width), from = low / kPageTokens;
+    if (dynamic) {
+      listed = early && last == p.pages;
+      share = (max(last - from, 0) + p.parts - 1) / p.parts;
+    }
+    pb = from + p.part * share;
+    pe = p.part == p.parts - 1 ? last : min(pb + share, last);
   }
 
   f32x4 o[NT][DT] = {};
@@ -341,7 +408,7 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
   };
 
   for (int p0 = pb + wave; p0 < pe; p0 += 256) {
-    if (!early || p0 != pb + wave) lp = list(p0 + 4 * lane, pe, page);
+    if (!listed || p0 != pb + wave) lp = list(p0 + 4 * lane, pe, page);
     if (page >= a.num_pages || lp * static_cast<int64_t>(kPageTokens) > pmax) page = -1;
     float ks, vs;
     page_scales(a, h, D, page, ks, vs);
@@ -430,15 +497,13 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
       f32x4 y = {};
 #pragma unroll
       for (int w = 0; w < 4; ++w) y += f[w] * *reinterpret_cast<const f32x4*>(&so[w][row][c]);
-      if (a.splits == 1) {
-        store_out4(a, t, hq, c, y, top, sum);
-      } else {
-        *reinterpret_cast<f32x4*>(a.ws_o + ((static_cast<int64_t>(split) * a.num_tokens + t) * a.heads + hq) * D + c) = y;
-      }
+      if (p.parts == 1) store_out4(a, t, hq, c, y, top, sum);
+      else *reinterpret_cast<f32x4*>(a.ws_o + (static_cast<int64_t>(blockIdx.x) * (16 * NT) + 16 * nt + row) * D + c) = y;
     }
     if ((tid & 15) == 0) {
-      if (a.splits == 1) store_lse(a, t, hq, top, sum);
-      else a.ws_ml[(static_cast<int64_t>(split) * a.num_tokens + t) * a.heads + hq] = make_float2(top, sum);
+      if (p.parts == 1) store_lse(a, t, hq, top, sum);
+      else a.ws_ml[blockIdx.x * (16 * NT) + 16 * nt + row] = make_float2(top, sum);
+      if (a.slots && p.part == 0) a.ws_rows[t * a.heads + hq] = make_int2(p.first, p.parts | (16 * nt + row) << 8);
     }
   }
 }
@@ -581,7 +646,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
     if (r >= rows) continue;
     const int64_t t = t0 + r / a.group;
     const int hq = h * a.group + r % a.group;
-    const int64_t at = (static_cast<int64_t>(split) * a.num_tokens + t) * a.heads + hq;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 128 + 32 * wave + 16 * nt + n;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       if (a.splits == 1) store_out4(a, t, hq, 16 * d + 4 * g, o[nt][d], m[nt], l[nt]);
@@ -590,15 +655,16 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
     if (g == 0) {
       if (a.splits == 1) store_lse(a, t, hq, m[nt], l[nt]);
       else a.ws_ml[at] = make_float2(m[nt], l[nt]);
+      if (a.slots && split == 0) a.ws_rows[t * a.heads + hq] = make_int2(unit, a.splits | (32 * wave + 16 * nt + n) << 8);
     }
   }
 }
 
-// Joins the splits: one wave per (token, head), lane s the s-th split's weight.
+// Joins a row's parts: one wave per (token, head), lane s the s-th part's weight.
 template <int D, bool LIST>
-__global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a) {
+__global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a, int slot_rows) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t = row / a.heads;
   const int hq = static_cast<int>(row - t * a.heads);
   if (t >= a.num_tokens) return;
@@ -607,9 +673,15 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a) {
   } else {
     if (t < a.qsl[0] || t >= a.qsl[a.num_seqs]) return;
   }
-  const int64_t step = static_cast<int64_t>(a.num_tokens) * a.heads;
+  const int2 info = a.ws_rows[row];
+  const int parts = info.y & 255, at = info.y >> 8;
+  // whole already; and a row that no workgroup took (more of them than the call said) names no part
+  if (parts < 2 || parts > kMaxSplits || at < 0 || at >= slot_rows || info.x < 0 ||
+      info.x + static_cast<int64_t>(parts - 1) * a.part_step >= a.slots)
+    return;
+  const int64_t first = static_cast<int64_t>(info.x) * slot_rows + at, step = static_cast<int64_t>(a.part_step) * slot_rows;
   float2 ml = make_float2(kNone, 0.0f);
-  if (lane < a.splits) ml = a.ws_ml[lane * step + row];
+  if (lane < parts) ml = a.ws_ml[first + lane * step];
   float top = ml.x;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
@@ -617,16 +689,15 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a) {
   float sum = f * ml.y;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m, 64);
-  // eight parts in flight; a split that saw nothing wrote none
-  const uint64_t some = __ballot(ml.y != 0.0f);
+  // eight parts in flight; the weight of one that saw nothing is 0
   const int c = 4 * (lane & (D / 4 - 1));
   f32x4 y = {};
-  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+  for (int s0 = 0; s0 < parts; s0 += 8) {
     f32x4 part[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       part[i] = f32x4{};
-      if ((some >> (s0 + i)) & 1) part[i] = *reinterpret_cast<const f32x4*>(a.ws_o + ((s0 + i) * step + row) * D + c);
+      if (s0 + i < parts) part[i] = *reinterpret_cast<const f32x4*>(a.ws_o + (first + (s0 + i) * step) * D + c);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) y += lane_value(f, s0 + i) * part[i];
@@ -640,12 +711,13 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a) {
 // ---------------------------------------------------------------------------
 struct GqaPlan {
   int row_tiles;  // 16-row tiles of a workgroup: 1, 2, 4 in every wave, or 8 over its four waves
-  int tiles, splits, split_pages;
-  int64_t units;
+  int tiles, splits, split_pages, budget;
+  int64_t units, slots;  // slots: workgroups
+  bool join;
 };
 
 // seqs: sequences (dense) or tokens (selected blocks); rows: query rows a kv
-// head has in each; pages(n): the most pages that n consecutive rows see.
+// head has in each; pages_of(n): the most pages that n consecutive rows see.
 template <typename Pages>
 static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int kv_heads, int dim, bool list, Pages pages_of) {
   GqaPlan p{};
@@ -654,18 +726,29 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int kv_heads, int dim, bool 
   p.tiles = static_cast<int>((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
   p.units = seqs * kv_heads * p.tiles;
   const int64_t pages = std::max<int64_t>(pages_of(std::min<int64_t>(rows, 16 * p.row_tiles)), 1);
-  // Workgroups wanted: sequences of a dense call differ in length, and the ones
-  // that a short sequence leaves empty are made up for by smaller parts (13
-  // sequences of 2,000 to 48,000 tokens, 8 kv heads of 128: 97 us at 768, 85 at
-  // 1,024, 82 at 2,048).  Lists are alike: one round of the chip is enough (32
-  // rows of 64 pages, 8 kv heads: 52 us at 768, 56 at 2,048), as for many rows.
-  const int64_t want = p.row_tiles == 8 ? 512 : list ? 768 : dim == 256 ? 1024 : 2048;
-  const int64_t least = p.row_tiles == 8 ? 16 : 4;  // pages of a split
-  int64_t splits = std::min<int64_t>({(want + p.units - 1) / std::max<int64_t>(p.units, 1), (pages + least - 1) / least,
+  // workgroups that run at once
+  const int64_t round = 256 * (p.row_tiles == 8 ? 2 : p.row_tiles * dim == 64 ? 4 : p.row_tiles * dim == 128 ? 3 : 2);
+  if (!list && p.row_tiles < 8 && seqs > 1 && seqs <= 64 && pages > 8) {
+    // Sequences of a dense call differ in length: their parts are shared out on
+    // the device, one round of the chip, or as many as leave two parts a unit
+    // (13 sequences of 2,000 to 48,000 tokens, 8 kv heads of 128: 82 us with
+    // 2,048 equal parts of the longest one, 72 so).
+    p.slots = round * std::max<int64_t>((2 * p.units + round - 1) / round, 1);
+    p.budget = static_cast<int>(p.slots / (kv_heads * static_cast<int64_t>(p.tiles)));
+    p.split_pages = static_cast<int>(std::min<int64_t>(pages, 1 << 30));
+    p.splits = 1;
+    p.join = true;
+    return p;
+  }
+  // One round: 32 rows of 64 listed pages, 8 kv heads: 52 us at 768, 56 at 2,048.
+  const int64_t least = p.row_tiles == 8 ? 16 : 4;  // pages of a part
+  int64_t splits = std::min<int64_t>({(round + p.units - 1) / std::max<int64_t>(p.units, 1), (pages + least - 1) / least,
                                       kMaxSplits});
   splits = std::max<int64_t>(splits, 1);
   p.split_pages = static_cast<int>((pages + splits - 1) / splits);
   p.splits = static_cast<int>((pages + p.split_pages - 1) / p.split_pages);
+  p.slots = p.units * p.splits;
+  p.join = p.splits > 1;
   return p;
 }
 
@@ -682,14 +765,14 @@ static GqaPlan block_plan(int64_t num_tokens, int group, int kv_heads, int dim, 
   return gqa_plan(num_tokens, group, kv_heads, dim, true, [&](int64_t) { return num_blocks; });
 }
 
+static int64_t rows_bytes(int64_t num_tokens, int64_t heads) { return (num_tokens * heads * 8 + 15) / 16 * 16; }
+
 static int64_t plan_bytes(const GqaPlan& p, int64_t num_tokens, int64_t heads, int64_t dim) {
-  return p.splits == 1 ? 0 : p.splits * num_tokens * heads * (dim + 2) * 4;
+  return p.join ? rows_bytes(num_tokens, heads) + p.slots * 16 * p.row_tiles * (dim + 2) * 4 : 0;
 }
 
 template <int D, bool LIST>
-static int launch_decode(const GqaAttnArgs& a, int row_tiles, hipStream_t s) {
-  const int64_t blocks = static_cast<int64_t>(a.units) * a.splits;
-  EKV_CHECK(blocks < (int64_t{1} << 31), "too many rows for one call");
+static int launch_decode(const GqaAttnArgs& a, int row_tiles, int64_t blocks, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(blocks));
   if constexpr (!LIST) {
     if (row_tiles == 8) {
@@ -708,16 +791,16 @@ static int launch_decode(const GqaAttnArgs& a, int row_tiles, hipStream_t s) {
     if (row_tiles == 4) gqa_decode_kernel<D, 4, LIST><<<grid, 256, 0, s>>>(a);
   }
   int rc = ekv_launch_status();
-  if (rc || a.splits == 1) return rc;
+  if (rc || !a.slots) return rc;
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.heads;
-  gqa_combine_kernel<D, LIST><<<dim3(static_cast<uint32_t>((rows + 3) / 4)), 256, 0, s>>>(a);
+  gqa_combine_kernel<D, LIST><<<dim3(static_cast<uint32_t>((rows + 3) / 4)), 256, 0, s>>>(a, 16 * row_tiles);
   return ekv_launch_status();
 }
 
 template <bool LIST>
 static int launch_attn(GqaAttnArgs& a, const GqaPlan& p, int dim, void* workspace, int64_t workspace_bytes,
                        void* stream) {
-  EKV_CHECK(p.units < (int64_t{1} << 31), "too many rows for one call");
+  EKV_CHECK(p.slots * 16 * p.row_tiles < (int64_t{1} << 31), "too many rows for one call");
   const int64_t need = plan_bytes(p, a.num_tokens, a.heads, dim);
   if (need > workspace_bytes || (need && !workspace)) {
     set_error("workspace too small");
@@ -725,12 +808,18 @@ static int launch_attn(GqaAttnArgs& a, const GqaPlan& p, int dim, void* workspac
   }
   EKV_CHECK(!need || aligned16(workspace), "workspace must be 16-byte aligned");
   a.tiles = p.tiles, a.units = static_cast<int32_t>(p.units), a.splits = p.splits, a.split_pages = p.split_pages;
-  a.ws_o = static_cast<float*>(workspace);
-  a.ws_ml = reinterpret_cast<float2*>(a.ws_o + static_cast<int64_t>(p.splits) * a.num_tokens * a.heads * dim);
+  a.budget = p.budget;
+  if (p.join) {
+    a.slots = static_cast<int32_t>(p.slots), a.part_step = p.budget ? a.kv_heads * p.tiles : a.units;
+    uint8_t* const ws = static_cast<uint8_t*>(workspace);
+    a.ws_rows = reinterpret_cast<int2*>(ws);
+    a.ws_o = reinterpret_cast<float*>(ws + rows_bytes(a.num_tokens, a.heads));
+    a.ws_ml = reinterpret_cast<float2*>(a.ws_o + p.slots * 16 * p.row_tiles * dim);
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dim == 64) return launch_decode<64, LIST>(a, p.row_tiles, s);
-  if (dim == 128) return launch_decode<128, LIST>(a, p.row_tiles, s);
-  return launch_decode<256, LIST>(a, p.row_tiles, s);
+  if (dim == 64) return launch_decode<64, LIST>(a, p.row_tiles, p.slots, s);
+  if (dim == 128) return launch_decode<128, LIST>(a, p.row_tiles, p.slots, s);
+  return launch_decode<256, LIST>(a, p.row_tiles, p.slots, s);
 }
 
 static int attn_args(GqaAttnArgs& a, const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride,
