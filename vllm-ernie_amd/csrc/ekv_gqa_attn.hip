@@ -15,7 +15,7 @@ namespace ekv {
 constexpr float kLog2e = 0x1.715476p+0f;
 constexpr float kLn2 = 0x1.62e430p-1f;
 constexpr float kNone = -1e30f;   // reference of a row that has seen no token
-constexpr float kSlack = 8.0f;    // log2 units over a row's reference that move it
+constexpr float kMoveAt = 4096.0f; // weight, or sum of a lane's 16, that moves a row's reference
 constexpr int kMaxSplits = 64;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -149,10 +149,12 @@ struct RowRange {
 
 // Scores x (token 16 j + 4 g + i of the page, row n) -> weights around the
 // rows' references m, as the B operand of the product with V, and their sums.
-// kscale > 0 takes a raw score to log2 units.  The references move only when a
-// score exceeds one by kSlack: weights stay below 2^kSlack, and most pages
-// need no maximum across lanes.  Masks are selects without branches.
-template <int NT, int DT>
+// kscale > 0 takes a raw score to log2 units.  A reference is a maximum that the
+// row has had, and moves only where the page's weights around it grow past
+// kMoveAt.  kBySum sees that in their sums, which costs no maximum but the raw
+// scores' registers (many rows: the products bound the kernel; 2,009 -> 1,950 us
+// at 4,096 rows); else in the largest score.  Masks are selects without branches.
+template <bool kBySum, int NT, int DT>
 __device__ __forceinline__ void softmax_page(f32x4 (&x)[NT][4], float kscale, bool whole, int first, int g,
                                              const RowRange<NT>& r, float (&m)[NT], float (&l)[NT],
                                              f32x4 (&o)[NT][DT], bf16x8 (&w)[NT][2]) {
@@ -170,22 +172,35 @@ __device__ __forceinline__ void softmax_page(f32x4 (&x)[NT][4], float kscale, bo
       }
     }
   }
-  float top[NT], most = kNone;
+  float y[NT][16], s[NT], top[NT], most = 0.0f;
+  auto largest = [&](int nt) {
+    float t = x[nt][0][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) t = fmaxf(t, x[nt][i >> 2][i & 3]);
+    return t * kscale;
+  };
+  auto weights = [&](int nt) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[nt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[nt][i >> 2][i & 3], kscale, -m[nt]));
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = y[nt][i] + y[nt][8 + i];
+    s[nt] = ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+  };
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    top[nt] = x[nt][0][0];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top[nt] = fmaxf(top[nt], x[nt][j][i]);
+    if (kBySum) {
+      weights(nt);
+      most = fmaxf(most, s[nt]);
+    } else {
+      top[nt] = largest(nt);
+      most = fmaxf(most, __builtin_amdgcn_exp2f(top[nt] - m[nt]));
     }
-    top[nt] *= kscale;
-    most = fmaxf(most, top[nt] - m[nt]);
   }
-  if (__any(most > kSlack)) {
+  if (__any(most > kMoveAt)) {  // infinite too: a row's first page, whose reference is none
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float t = fmaxf(top[nt], m[nt]);
+      float t = fmaxf(kBySum ? largest(nt) : top[nt], m[nt]);
       t = fmaxf(t, __shfl_xor(t, 16, 64));
       t = fmaxf(t, __shfl_xor(t, 32, 64));
       const float f = __builtin_amdgcn_exp2f(m[nt] - t);
@@ -193,19 +208,15 @@ __device__ __forceinline__ void softmax_page(f32x4 (&x)[NT][4], float kscale, bo
       l[nt] *= f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[nt][d] *= f;
+      if (kBySum) weights(nt);
     }
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    if (!kBySum) weights(nt);
+    l[nt] += s[nt];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[nt][j][i], kscale, -m[nt]));
-        l[nt] += y;
-        w[nt][j >> 1][4 * (j & 1) + i] = static_cast<__bf16>(y);
-      }
-    }
+    for (int i = 0; i < 16; ++i) w[nt][i >> 3][i & 7] = static_cast<__bf16>(y[nt][i]);
   }
 }
 
@@ -446,7 +457,7 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
       __builtin_amdgcn_sched_barrier(0);
       const bool whole = first + kPageTokens - 1 <= rr.pany && (!a.window || first > pmax - a.window);
       bf16x8 w[NT][2];
-      softmax_page<NT, DT>(x, kscale, whole, first, g, rr, m, l, o, w);
+      softmax_page<false, NT, DT>(x, kscale, whole, first, g, rr, m, l, o, w);
       if (!whole) {
         const uint4 keep = v_keep(first, low, pmax, g);
 #pragma unroll
@@ -609,23 +620,26 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
       if (first <= rr.pmax && first + kPageTokens > wave_low) {
         const bf16x8* const src = buf + half * kHalf + lane;
         f32x4 x[NT][4] = {};
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int s = 0; s < 2 * S; ++s) {
 #pragma unroll
-          for (int s = 0; s < 2 * S; ++s) {
+          for (int j = 0; j < 4; ++j) {
             const bf16x8 k = src[(j * 2 * S + s) * 64];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               x[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[nt][s], x[nt][j], 0, 0, 0);
           }
         }
+        __builtin_amdgcn_s_setprio(0);
         const bool whole = first + kPageTokens - 1 <= rr.pany && (!a.window || first > rr.pmax - a.window);
         bf16x8 w[NT][2];
-        softmax_page<NT, DT>(x, lane_value(ks, at), whole, first, g, rr, m, l, o, w);
+        softmax_page<true, NT, DT>(x, lane_value(ks, at), whole, first, g, rr, m, l, o, w);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+          for (int d = 0; d < DT; ++d) {
             const bf16x8 v = src[(8 * S + 2 * d + u) * 64];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -633,6 +647,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
           }
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       if (next >= 0) stage(next, half ^ 1);
       at = next, half ^= 1;
     }
