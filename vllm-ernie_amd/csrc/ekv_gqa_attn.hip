@@ -756,7 +756,11 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int kv_heads, int dim, bool 
     return p;
   }
   // One round: 32 rows of 64 listed pages, 8 kv heads: 52 us at 768, 56 at 2,048.
-  const int64_t least = p.row_tiles == 8 ? 16 : 4;  // pages of a part
+  // Pages of a part.  Of many rows: shorter parts where units are fewer than CUs
+  // (4 sequences of 4,096 tokens, 16 rows, 8 kv heads of 128: 37 us at 16, 31 at
+  // 8), longer ones where each CU has one already (32 of 1,000: 50 us in two
+  // parts of 8, 35 in one).
+  const int64_t least = p.row_tiles < 8 ? 4 : p.units < 256 ? 8 : 32;
   int64_t splits = std::min<int64_t>({(round + p.units - 1) / std::max<int64_t>(p.units, 1), (pages + least - 1) / least,
                                       kMaxSplits});
   splits = std::max<int64_t>(splits, 1);
