@@ -852,7 +852,7 @@ static int attn_args(GqaAttnArgs& a, const uint16_t* q, int64_t q_tok_stride, in
   EKV_CHECK(scale > 0.0f, "scale must be positive");
   a = GqaAttnArgs{};
   if (!num_tokens || !num_seqs) return kOk;
-  EKV_CHECK(q && cache && block_table && positions && out, "null pointer");
+  EKV_CHECK(q && (cache || !num_pages) && (block_table || !bt_width) && positions && out, "null pointer");
   EKV_CHECK(page_stride >= gqa_page_bytes(kv_heads, dim) && page_stride % 16 == 0 && aligned16(cache),
             "page_stride must be a multiple of 16 of at least kv_heads * (128 * dim + 8) bytes");
   EKV_CHECK(aligned8(out) && out_tok_stride % 4 == 0 && out_head_stride % 4 == 0,

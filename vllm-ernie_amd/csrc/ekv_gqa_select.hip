@@ -307,7 +307,7 @@ extern "C" int ekv_gqa_block_select(const uint16_t* q, int64_t q_tok_stride, int
             "keep_first + keep_last must be at most num_blocks");
   EKV_CHECK(max_len <= kSelMaxBlocks * kPageTokens, "max_len must be at most 2097152 tokens");
   if (!num_tokens || !num_seqs || !num_blocks) return kOk;
-  EKV_CHECK(q && summary && block_table && positions && req_ids && blocks, "null pointer");
+  EKV_CHECK(q && (summary || !num_pages) && (block_table || !bt_width) && positions && req_ids && blocks, "null pointer");
   EKV_CHECK(summary_stride >= gqa_summary_bytes(kv_heads, dim) && summary_stride % 16 == 0 && aligned16(summary),
             "summary_stride must be a multiple of 16 of at least kv_heads * (dim + 4) bytes");
   EKV_CHECK(num_pages < (int64_t{1} << 31), "too many pages");

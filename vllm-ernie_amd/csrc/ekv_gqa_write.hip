@@ -550,7 +550,7 @@ static int append_args(GqaAppendArgs& a, const uint16_t* k, int64_t k_tok_stride
   EKV_CHECK(kv_heads > 0 && num_tokens >= 0 && num_seqs >= 0 && max_query_len >= 0, "negative sizes");
   a = GqaAppendArgs{};
   if (!num_tokens || !num_seqs || !max_query_len) return kOk;
-  EKV_CHECK(k && v && positions && qsl && block_table && cache, "null pointer");
+  EKV_CHECK(k && v && positions && qsl && (block_table || !bt_width) && (cache || !num_pages), "null pointer");
   EKV_CHECK(bt_width >= 0 && num_pages >= 0, "negative sizes");
   EKV_CHECK(page_stride >= gqa_page_bytes(kv_heads, dim) && page_stride % 16 == 0 && aligned16(cache),
             "page_stride must be a multiple of 16 of at least kv_heads * (128 * dim + 8) bytes");

@@ -1093,45 +1093,54 @@ def _refuse(msg: str) -> None:
 
 
 def _gqa_device(*ts: torch.Tensor | None) -> int:
+    """The one device of all tensors."""
     dev = ts[0].get_device()
-    for t in ts:
-        if t is not None and t.get_device() != dev:
-            _check_dev(*ts)
-            _refuse("tensors on different devices")
-    if dev < 0:
+    if dev < 0 or any([t is not None and t.get_device() != dev for t in ts]):
         _check_dev(*ts)
+        _refuse("tensors on different devices")
     return dev
 
 
+_gqa_functions: dict = {}
+
+
 def _gqa_call(dev: int, name: str, *args) -> None:
-    stream = torch._C._cuda_getCurrentRawStream(dev)
+    fn = _gqa_functions.get(name)
+    if fn is None:
+        fn = _gqa_functions[name] = getattr(_lib.load(), name)
     if dev == torch.cuda.current_device():
-        _lib.call(name, *args, stream)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        raise _lib.EkvError(f"{name} failed ({rc}): {_lib.load().ekv_last_error().decode(errors='replace')}")
 
 
 def _heads3(t: torch.Tensor, what: str) -> tuple:
-    """(T, heads, D, token stride, head stride) of bf16 rows; the stride of a
-    dim of one entry, which no address depends on, is the packed one."""
+    """(T, heads, D, address, token stride, head stride) of bf16 rows; the
+    stride of a dim of one entry, which no address depends on, is the packed one."""
     if t.dtype is not torch.bfloat16:
         _refuse(f"{what} bf16 [T, heads, D]: expected bfloat16, got {t.dtype}")
-    if t.dim() != 3:
+    try:
+        T, H, D = t.shape
+    except ValueError:
         _refuse(f"{what} [T, heads, D]")
-    T, H, D = t.shape
     s0, s1, s2 = t.stride()
     if s2 != 1 and D > 1:
         _refuse(f"{what} [T, heads, D] with unit channel stride")
-    return T, H, D, s0 if T > 1 else H * D, s1 if H > 1 else D
+    return T, H, D, t.data_ptr(), s0 if T > 1 else H * D, s1 if H > 1 else D
 
 
 def _bytes2(t: torch.Tensor, what: str) -> tuple:
     """(address, row stride, rows) of uint8 [rows, bytes]."""
-    if t.dtype is not torch.uint8 or t.dim() != 2 or t.stride(1) != 1:
-        _refuse(f"{what} uint8 [pages, bytes] with unit byte stride")
+    if t.dtype is not torch.uint8 or t.dim() != 2:
+        _refuse(f"{what} uint8 [pages, bytes]")
     n, w = t.shape
-    return t.data_ptr(), t.stride(0) if n > 1 else w, n
+    s0, s1 = t.stride()
+    if s1 != 1:
+        _refuse(f"{what} uint8 [pages, bytes] with unit byte stride")
+    return t.data_ptr(), s0 if n > 1 else w, n
 
 
 def _table(t: torch.Tensor, rows: int) -> tuple:
@@ -1147,7 +1156,7 @@ def _table(t: torch.Tensor, rows: int) -> tuple:
 
 def _vector(t: torch.Tensor, dtype, n: int, what: str) -> int:
     """Address of a contiguous vector of at least n entries."""
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
+    if t.dtype is not dtype or t.numel() < n or t.dim() != 1 or not t.is_contiguous():
         _refuse(f"{what} {dtype} [{n}] contiguous")
     return t.data_ptr()
 
@@ -1177,7 +1186,7 @@ def _block_attention_bytes(*sizes: int) -> int:
 def _weight(w: torch.Tensor | None, dim: int) -> int | None:
     if w is None:
         return None
-    if w.dtype not in (torch.float32, torch.bfloat16) or w.dim() != 1 or w.shape[0] != dim or not w.is_contiguous():
+    if w.dtype not in (torch.float32, torch.bfloat16) or w.dim() != 1 or w.numel() != dim or not w.is_contiguous():
         _refuse("norm weights fp32 or bf16 [D] contiguous")
     return w.data_ptr()
 
@@ -1204,32 +1213,32 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_w: torch.Tensor | None, k_w
     on pairs half the slice apart or, ``interleaved``, neighbours; fp32,
     rounded once.  Returns new contiguous ``(q, k)``."""
     dev = _gqa_device(q, k, q_w, k_w, cos_sin, positions)
-    T, H, D, q0, q1 = _heads3(q, "q")
-    Tk, KV, Dk, k0, k1 = _heads3(k, "k")
+    T, H, D, qp, q0, q1 = _heads3(q, "q")
+    Tk, KV, Dk, kp, k0, k1 = _heads3(k, "k")
     if T != Tk or D != Dk:
         _refuse("k must be [T, H_kv, D] like q")
     pos = _vector(positions, torch.int64, T, "positions")
     norm = _norm_args(q_w, k_w, D, eps, cos_sin, rope_offset, interleaved)
     q_out, k_out = q.new_empty((T, H, D)), k.new_empty((T, KV, D))
-    _gqa_call(dev, "ekv_qk_norm_rope", q.data_ptr(), q0, q1, H, k.data_ptr(), k0, k1, KV, T, D, *norm, pos,
+    _gqa_call(dev, "ekv_qk_norm_rope", qp, q0, q1, H, kp, k0, k1, KV, T, D, *norm, pos,
               q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
 def _append_args(k, v, positions, qsl, max_query_len, block_table, cache, summary) -> tuple:
-    T, KV, D, k0, k1 = _heads3(k, "k")
-    Tv, KVv, Dv, v0, v1 = _heads3(v, "v")
+    T, KV, D, kp, k0, k1 = _heads3(k, "k")
+    Tv, KVv, Dv, vp, v0, v1 = _heads3(v, "v")
     if T != Tv or KV != KVv or D != Dv:
         _refuse("v must be [T, H_kv, D] like k")
     pos, seqs = _vector(positions, torch.int64, T, "positions"), _vector(qsl, torch.int32, 1, "qsl")
-    B = qsl.shape[0] - 1
+    B = qsl.numel() - 1
     c, c0, pages = _bytes2(cache, "cache")
     s = s0 = 0
     if summary is not None:
         s, s0, records = _bytes2(summary, "summary")
         if records < pages:
             _refuse("summary needs a record for each page")
-    return ((k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, T, KV, D),
+    return ((kp, k0, k1, vp, v0, v1, T, KV, D),
             (pos, seqs, B, max_query_len, *_table(block_table, B), c, c0, pages, s, s0))
 
 
@@ -1251,21 +1260,21 @@ def gqa_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_w: torch.T
     """``qk_norm_rope`` of q and k and ``gqa_append`` of the prepared keys and
     ``v`` in one launch, same bytes; returns the prepared ``q``."""
     dev = _gqa_device(q, k, v, q_w, k_w, cos_sin, positions, qsl, block_table, cache, summary)
-    T, H, D, q0, q1 = _heads3(q, "q")
+    T, H, D, qp, q0, q1 = _heads3(q, "q")
     head, tail = _append_args(k, v, positions, qsl, max_query_len, block_table, cache, summary)
     if head[6] != T or head[8] != D:
         _refuse("k must be [T, H_kv, D] like q")
     norm = _norm_args(q_w, k_w, D, eps, cos_sin, rope_offset, interleaved)
     q_out = q.new_empty((T, H, D))
-    _gqa_call(dev, "ekv_gqa_prologue", q.data_ptr(), q0, q1, H, *head, *norm, *tail, q_out.data_ptr())
+    _gqa_call(dev, "ekv_gqa_prologue", qp, q0, q1, H, *head, *norm, *tail, q_out.data_ptr())
     return q_out
 
 
 def _gqa_attn_args(q, cache, kv_heads, block_table, seqs, positions, out, lse, sinks) -> tuple:
-    T, H, D, q0, q1 = _heads3(q, "q")
+    T, H, D, qp, q0, q1 = _heads3(q, "q")
     if kv_heads <= 0 or H % kv_heads:
         _refuse("heads must be a multiple of kv_heads")
-    To, Ho, Do, o0, o1 = _heads3(out, "out")
+    To, Ho, Do, op, o0, o1 = _heads3(out, "out")
     if To != T or Ho != H or Do != D:
         _refuse("out bf16 [T, H, D] like q")
     l = l0 = 0
@@ -1274,8 +1283,8 @@ def _gqa_attn_args(q, cache, kv_heads, block_table, seqs, positions, out, lse, s
             _refuse("lse fp32 [T, H]")
         l, l0 = lse.data_ptr(), lse.stride(0)
     s = None if sinks is None else _vector(sinks, torch.float32, H, "sinks")
-    return (T, H, D, (q.data_ptr(), q0, q1, T, H, kv_heads, D, *_bytes2(cache, "cache"), *_table(block_table, seqs),
-                      _vector(positions, torch.int64, T, "positions")), s, (out.data_ptr(), o0, o1, l, l0))
+    return (T, H, D, (qp, q0, q1, T, H, kv_heads, D, *_bytes2(cache, "cache"), *_table(block_table, seqs),
+                      _vector(positions, torch.int64, T, "positions")), s, (op, o0, o1, l, l0))
 
 
 def _gqa_workspace(workspace, need: int, like: torch.Tensor) -> tuple:
@@ -1306,7 +1315,7 @@ def gqa_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, block_tab
     Rows that see nothing get zeros and -inf, rows of no sequence stay."""
     dev = _gqa_device(q, cache, block_table, positions, qsl, out, lse, sinks, workspace)
     seqs = _vector(qsl, torch.int32, 1, "qsl")
-    B = qsl.shape[0] - 1
+    B = qsl.numel() - 1
     T, H, D, head, sink, tail = _gqa_attn_args(q, cache, kv_heads, block_table, B, positions, out, lse, sinks)
     ws, ws_bytes, workspace = _gqa_workspace(
         workspace, _attention_bytes(T, B, max_query_len, max_len, H, kv_heads, D, window), q)
@@ -1330,10 +1339,10 @@ def gqa_block_select(q: torch.Tensor, summary: torch.Tensor, kv_heads: int, bloc
     the largest score against their mean keys, ascending, -1 behind them; the
     first ``keep_first`` and the last ``keep_last`` pages come before others."""
     dev = _gqa_device(q, summary, block_table, positions, req_ids, blocks)
-    T, H, D, q0, q1 = _heads3(q, "q")
+    T, H, D, qp, q0, q1 = _heads3(q, "q")
     if kv_heads <= 0 or H % kv_heads:
         _refuse("heads must be a multiple of kv_heads")
-    _gqa_call(dev, "ekv_gqa_block_select", q.data_ptr(), q0, q1, T, H, kv_heads, D, *_bytes2(summary, "summary"),
+    _gqa_call(dev, "ekv_gqa_block_select", qp, q0, q1, T, H, kv_heads, D, *_bytes2(summary, "summary"),
               *_table(block_table, 0), _vector(positions, torch.int64, T, "positions"),
               _vector(req_ids, torch.int32, T, "req_ids"), block_table.shape[0], max_len, keep_first, keep_last,
               *_block_lists(blocks, T, kv_heads))
