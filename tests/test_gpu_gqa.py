@@ -502,6 +502,31 @@ def test_step_graph_replay_and_streams(dev):
         assert torch.equal(layer.d_cache, want[1]) and torch.equal(layer.d_summary, want[2]), f"replay {rep}"
 
 
+def test_torch_operators_are_the_wrappers(dev):
+    """torch.ops.ernie_kv.*: the wrappers' bytes."""
+    import ernie_kv.torch_ops  # noqa: F401
+    from ernie_kv import ops
+
+    rng = np.random.default_rng(33)
+    H, n = 8, 5
+    layer = Layer(dev, rng, [500, 70], 2, 64, extra=8)
+    clean = layer.d_cache.clone(), layer.d_summary.clone()
+    st = step_state(dev, rng, layer, [2, 1], H, n)
+    outs, got = ("o1", "l1", "o2", "l2", "ids"), []
+    for o in (ops, torch.ops.ernie_kv):
+        layer.d_cache.copy_(clean[0]), layer.d_summary.copy_(clean[1])
+        for k in outs:
+            st[k].fill_(7)
+        q, k = o.qk_norm_rope(st["q"], st["k"], st["w"], st["w"], 1e-6, st["cs"], st["pos"])
+        o.gqa_append(k, st["v"], st["pos"], st["qsl"], st["most"], layer.d_bt, layer.d_cache, layer.d_summary)
+        first = layer.d_cache.clone()
+        layer.d_cache.copy_(clean[0])
+        run_step(o, layer, st, workspaces(ops, st, layer, H, n, dev))
+        assert torch.equal(first, layer.d_cache)
+        got.append([q, k, layer.d_cache.clone(), layer.d_summary.clone()] + [st[x].clone() for x in outs])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and not torch.equal(got[0][2], clean[0])
+
+
 def test_wrappers_refuse(dev):
     from ernie_kv import _lib, ops
 

@@ -212,3 +212,27 @@ def test_wrappers_refuse_cpu_tensors():
         ops.gqa_attention(z, cache, 1, i[None], p, i, 1, 64, 1.0, torch.empty_like(z))
     with pytest.raises(ValueError, match="device tensors"):
         ops.qk_norm_rope(z, z, None, None, 1e-6, None, p)
+
+
+def test_torch_ops_registered_and_traced():
+    """The operators name what they write, and their fakes give what they return, without a launch."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import ernie_kv.torch_ops as T
+
+    writes = {"qk_norm_rope": set(), "gqa_append": {"cache", "summary"}, "gqa_prologue": {"cache", "summary"},
+              "gqa_attention": {"out", "lse", "workspace"}, "gqa_block_select": {"blocks"},
+              "gqa_block_attention": {"out", "lse", "workspace"}}
+    assert set(T.GQA_OPS) == set(writes)
+    for name, expect in writes.items():
+        schema = getattr(torch.ops.ernie_kv, name).default._schema
+        assert {a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write} == expect, name
+    with FakeTensorMode():
+        q, k = torch.empty((3, 8, 64), dtype=torch.bfloat16), torch.empty((3, 2, 64), dtype=torch.bfloat16)
+        pos, i = torch.empty(3, dtype=torch.int64), torch.empty(4, dtype=torch.int32)
+        a, b = torch.ops.ernie_kv.qk_norm_rope(q[:, ::2], k, None, None, 1e-6, None, pos)
+        assert a.shape == (3, 4, 64) and a.is_contiguous() and b.shape == k.shape
+        cache = torch.empty((4, 2 * 128 * 64 + 16), dtype=torch.uint8)
+        y = torch.ops.ernie_kv.gqa_prologue(q, k, k, None, None, 1e-6, None, pos, i, 1, i[None], cache, None)
+        assert y.shape == q.shape and y.dtype == q.dtype
+        assert torch.ops.ernie_kv.gqa_attention(q, cache, 2, i[None], pos, i, 1, 64, 0.1, y, None, None) is None

@@ -115,3 +115,75 @@ def _no_output(*args, **kwargs) -> None:
 
 for _name in OPS:
     globals()[_name].register_fake(_no_output)
+
+
+# --------------------------------------------------------------------------- grouped-query layers
+# The dispatcher counts the versions of the tensors an operator writes by their
+# places, so those are always passed, None where there is none.
+@torch.library.custom_op(f"{_NS}::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[torch.Tensor],
+                 eps: float, cos_sin: Optional[torch.Tensor], positions: torch.Tensor, interleaved: bool = False,
+                 rope_offset: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of each q / k head and the rotation of a slice of its channels."""
+    return ops.qk_norm_rope(q, k, q_w, k_w, eps, cos_sin, positions, interleaved, rope_offset)
+
+
+@qk_norm_rope.register_fake
+def _(q, k, q_w, k_w, eps, cos_sin, positions, interleaved=False, rope_offset=0):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op(f"{_NS}::gqa_append", mutates_args=("cache", "summary"))
+def gqa_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, qsl: torch.Tensor, max_query_len: int,
+               block_table: torch.Tensor, cache: torch.Tensor, summary: Optional[torch.Tensor]) -> None:
+    """Keys and values into 8-bit pages with a scale per (page, kv head)."""
+    ops.gqa_append(k, v, positions, qsl, max_query_len, block_table, cache, summary)
+
+
+@torch.library.custom_op(f"{_NS}::gqa_prologue", mutates_args=("cache", "summary"))
+def gqa_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_w: Optional[torch.Tensor],
+                 k_w: Optional[torch.Tensor], eps: float, cos_sin: Optional[torch.Tensor], positions: torch.Tensor,
+                 qsl: torch.Tensor, max_query_len: int, block_table: torch.Tensor, cache: torch.Tensor,
+                 summary: Optional[torch.Tensor], interleaved: bool = False, rope_offset: int = 0) -> torch.Tensor:
+    """``qk_norm_rope`` and ``gqa_append`` in one launch; the prepared q."""
+    return ops.gqa_prologue(q, k, v, q_w, k_w, eps, cos_sin, positions, qsl, max_query_len, block_table, cache, summary,
+                            interleaved, rope_offset)
+
+
+@gqa_prologue.register_fake
+def _(q, k, v, q_w, k_w, eps, cos_sin, positions, qsl, max_query_len, block_table, cache, summary,
+      interleaved=False, rope_offset=0):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{_NS}::gqa_attention", mutates_args=("out", "lse", "workspace"))
+def gqa_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, block_table: torch.Tensor,
+                  positions: torch.Tensor, qsl: torch.Tensor, max_query_len: int, max_len: int, scale: float,
+                  out: torch.Tensor, lse: Optional[torch.Tensor], workspace: Optional[torch.Tensor],
+                  sinks: Optional[torch.Tensor] = None, window: int = 0) -> None:
+    """Causal attention over the 8-bit pages of each sequence."""
+    ops.gqa_attention(q, cache, kv_heads, block_table, positions, qsl, max_query_len, max_len, scale, out, lse, sinks,
+                      window, workspace)
+
+
+@torch.library.custom_op(f"{_NS}::gqa_block_select", mutates_args=("blocks",))
+def gqa_block_select(q: torch.Tensor, summary: torch.Tensor, kv_heads: int, block_table: torch.Tensor,
+                     positions: torch.Tensor, req_ids: torch.Tensor, max_len: int, blocks: torch.Tensor,
+                     keep_first: int = 1, keep_last: int = 2) -> None:
+    """The pages with the largest scores against their mean keys, for each row and kv head."""
+    ops.gqa_block_select(q, summary, kv_heads, block_table, positions, req_ids, max_len, blocks, keep_first, keep_last)
+
+
+@torch.library.custom_op(f"{_NS}::gqa_block_attention", mutates_args=("out", "lse", "workspace"))
+def gqa_block_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, block_table: torch.Tensor,
+                        positions: torch.Tensor, req_ids: torch.Tensor, blocks: torch.Tensor, scale: float,
+                        out: torch.Tensor, lse: Optional[torch.Tensor], workspace: Optional[torch.Tensor],
+                        sinks: Optional[torch.Tensor] = None) -> None:
+    """``gqa_attention`` over the listed pages."""
+    ops.gqa_block_attention(q, cache, kv_heads, block_table, positions, req_ids, blocks, scale, out, lse, sinks,
+                            workspace)
+
+
+GQA_OPS = ("qk_norm_rope", "gqa_append", "gqa_prologue", "gqa_attention", "gqa_block_select", "gqa_block_attention")
+for _name in ("gqa_append", "gqa_attention", "gqa_block_select", "gqa_block_attention"):
+    globals()[_name].register_fake(_no_output)
