@@ -521,18 +521,25 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
 
 // ---------------------------------------------------------------------------
 // Many rows a kv head: one workgroup per (128 rows, kv head, range of pages).
-// Its 4 waves hold 32 rows each and share every page: each wave brings a
-// quarter of it, converted to bf16 once, into LDS in the order of the operands
+// Its waves (4 of 32 rows; 8 of 16 at 256 channels, whose sums of 32 would leave
+// one wave a SIMD: 1,490 -> 1,100 us at 2,048 rows) share every page: each brings
+// its part of it, converted to bf16 once, into LDS in the order of the operands
 // (1 KB reads of 64 consecutive 16-byte pieces), while the page before is
 // multiplied.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaAttnArgs a) {
-  constexpr int S = D / 64, DT = D / 16, VT = DT / 4, NT = 2;
+struct PrefillShape {
+  static constexpr int kWaves = D == 256 ? 8 : 4, kTiles = 8 / kWaves;  // 16-row tiles of a wave
+};
+
+template <int D>
+__global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_kernel(GqaAttnArgs a) {
+  constexpr int W = PrefillShape<D>::kWaves, NT = PrefillShape<D>::kTiles;
+  constexpr int S = D / 64, DT = D / 16, KT = 4 * S / W, VT = DT / W;  // pieces of K and V that a wave brings
   constexpr int kHalf = (8 * S + 2 * DT) * 64;  // 16-byte pieces of a page: K, then V
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   bf16x8* const buf = reinterpret_cast<bf16x8*>(smem);
-  __shared__ int ranges[4][2];
+  __shared__ int ranges[W][2];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int unit = static_cast<int>(blockIdx.x) % a.units, split = static_cast<int>(blockIdx.x) / a.units;
@@ -541,7 +548,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
   const int t0 = a.qsl[b];
   const int rows = (min(a.qsl[b + 1], a.num_tokens) - t0) * a.group;
   if (t0 < 0 || tile * 128 >= rows) return;
-  const int r0 = tile * 128 + 32 * wave;
+  const int r0 = tile * 128 + 16 * NT * wave;
   RowRange<NT> rr;
   bf16x8 q[NT][2 * S];
 #pragma unroll
@@ -551,7 +558,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
   __syncthreads();
   int pmax = -1, pmin = 0x7fffffff;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) pmax = max(pmax, ranges[w][0]), pmin = min(pmin, ranges[w][1]);
+  for (int w = 0; w < W; ++w) pmax = max(pmax, ranges[w][0]), pmin = min(pmin, ranges[w][1]);
   pmax = __builtin_amdgcn_readfirstlane(pmax);
   pmin = __builtin_amdgcn_readfirstlane(pmin);
   const int low = a.window && pmax >= 0 ? max(pmin - a.window + 1, 0) : 0;
@@ -565,12 +572,14 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) m[nt] = kNone, l[nt] = 0.0f;
 
-  // this wave's quarter of a page: tokens 16 wave .. of K, channels D / 4 wave .. of V
+  // this wave's part of a page: pieces KT wave .. of K (S of each 16 tokens),
+  // channels D / W wave .. of V
   const uint8_t* const k_base = a.cache + static_cast<int64_t>(h) * kPageTokens * D;
   const uint32_t v_step = static_cast<uint32_t>(a.kv_heads) * kPageTokens * D;
-  const uint32_t k_at = (16 * wave + n) * D + 16 * g, v_at = (D / 4 * wave + n) * kPageTokens + 16 * g;
+  const uint32_t k_at = (16 * (KT * wave / S) + n) * D + 64 * (KT * wave % S) + 16 * g;
+  const uint32_t v_at = (D / W * wave + n) * kPageTokens + 16 * g;
   const int32_t* bt = a.block_table + b * a.bt_stride;
-  uint4 kr[S], vr[VT];
+  uint4 kr[KT], vr[VT];
 
   for (int p0 = pb; p0 < pe; p0 += 64) {
     float ks, vs;
@@ -583,7 +592,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
       const uint8_t* pg = k_base + static_cast<int64_t>(__builtin_amdgcn_readlane(page, at)) * a.page_stride;
       const PageRsrc rk = page_rsrc(pg, kPageTokens * D), rv = page_rsrc(pg + v_step, kPageTokens * D);
 #pragma unroll
-      for (int s = 0; s < S; ++s) kr[s] = load16(rk, k_at + 64 * s, 0);
+      for (int s = 0; s < KT; ++s) kr[s] = load16(rk, k_at + 64 * s, 0);
 #pragma unroll
       for (int i = 0; i < VT; ++i) vr[i] = load16(rv, v_at + 16 * i * kPageTokens, 0);
     };
@@ -592,9 +601,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
       const int first = (p0 + at) * kPageTokens;
       const float vscale = lane_value(vs, at);
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        dst[((wave * S + s) * 2) * 64] = fp8x8_to_bf16(kr[s].x, kr[s].y, 1.0f);
-        dst[((wave * S + s) * 2 + 1) * 64] = fp8x8_to_bf16(kr[s].z, kr[s].w, 1.0f);
+      for (int s = 0; s < KT; ++s) {
+        dst[((wave * KT + s) * 2) * 64] = fp8x8_to_bf16(kr[s].x, kr[s].y, 1.0f);
+        dst[((wave * KT + s) * 2 + 1) * 64] = fp8x8_to_bf16(kr[s].z, kr[s].w, 1.0f);
       }
       if (first + kPageTokens - 1 > pmax || first < low) {
         const uint4 keep = v_keep(first, low, pmax, g);
@@ -661,7 +670,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
     if (r >= rows) continue;
     const int64_t t = t0 + r / a.group;
     const int hq = h * a.group + r % a.group;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 128 + 32 * wave + 16 * nt + n;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 128 + 16 * NT * wave + 16 * nt + n;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       if (a.splits == 1) store_out4(a, t, hq, 16 * d + 4 * g, o[nt][d], m[nt], l[nt]);
@@ -670,7 +679,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) gqa_prefill_kernel(GqaA
     if (g == 0) {
       if (a.splits == 1) store_lse(a, t, hq, m[nt], l[nt]);
       else a.ws_ml[at] = make_float2(m[nt], l[nt]);
-      if (a.slots && split == 0) a.ws_rows[t * a.heads + hq] = make_int2(unit, a.splits | (32 * wave + 16 * nt + n) << 8);
+      if (a.slots && split == 0) a.ws_rows[t * a.heads + hq] = make_int2(unit, a.splits | (16 * (NT * wave + nt) + n) << 8);
     }
   }
 }
@@ -737,7 +746,7 @@ template <typename Pages>
 static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int kv_heads, int dim, bool list, Pages pages_of) {
   GqaPlan p{};
   const int most = dim == 256 ? 1 : dim == 128 ? 2 : 4;
-  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : rows <= 64 || list ? most : 8;
+  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : rows <= (dim == 256 ? 48 : 64) || list ? most : 8;
   p.tiles = static_cast<int>((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
   p.units = seqs * kv_heads * p.tiles;
   const int64_t pages = std::max<int64_t>(pages_of(std::min<int64_t>(rows, 16 * p.row_tiles)), 1);
@@ -799,7 +808,7 @@ static int launch_decode(const GqaAttnArgs& a, int row_tiles, int64_t blocks, hi
       if (kBytes >= 65536)
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(gqa_prefill_kernel<D>),
                                   hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-      gqa_prefill_kernel<D><<<grid, 256, kBytes, s>>>(a);
+      gqa_prefill_kernel<D><<<grid, 64 * PrefillShape<D>::kWaves, kBytes, s>>>(a);
     }
   }
   if (row_tiles == 1) gqa_decode_kernel<D, 1, LIST><<<grid, 256, 0, s>>>(a);
