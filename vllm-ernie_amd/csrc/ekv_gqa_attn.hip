@@ -126,9 +126,10 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
 }
 
 // Result of a row whose weights sum to l around the reference m: 4 channels.
-__device__ __forceinline__ void store_out4(const GqaAttnArgs& a, int64_t t, int hq, int c, f32x4 o, float m, float l) {
+__device__ __forceinline__ void store_out4(const GqaAttnArgs& a, int64_t t, int hq, int c, f32x4 o, float m, float l,
+                                           float sink) {
   float den = l;
-  if (a.sinks) den += __builtin_amdgcn_exp2f(a.sinks[hq] * kLog2e - m);
+  if (a.sinks) den += __builtin_amdgcn_exp2f(sink * kLog2e - m);
   const float inv = den > 0.0f ? 1.0f / den : (den == den ? 0.0f : den);
   const uint32_t lo = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(o[0] * inv), static_cast<__bf16>(o[1] * inv)});
   const uint32_t hi = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(o[2] * inv), static_cast<__bf16>(o[3] * inv)});
@@ -495,6 +496,7 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
     if (r >= rows) continue;
     const int64_t t = t0 + r / a.group;
     const int hq = h * a.group + r % a.group;
+    const float sink = a.sinks ? a.sinks[hq] : 0.0f;
     float top = kNone, sum = 0.0f, f[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) top = fmaxf(top, sml[w][row].x);
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
       f32x4 y = {};
 #pragma unroll
       for (int w = 0; w < 4; ++w) y += f[w] * *reinterpret_cast<const f32x4*>(&so[w][row][c]);
-      if (p.parts == 1) store_out4(a, t, hq, c, y, top, sum);
+      if (p.parts == 1) store_out4(a, t, hq, c, y, top, sum, sink);
       else *reinterpret_cast<f32x4*>(a.ws_o + (static_cast<int64_t>(blockIdx.x) * (16 * NT) + 16 * nt + row) * D + c) = y;
     }
     if ((tid & 15) == 0) {
@@ -670,10 +672,11 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
     if (r >= rows) continue;
     const int64_t t = t0 + r / a.group;
     const int hq = h * a.group + r % a.group;
+    const float sink = a.sinks ? a.sinks[hq] : 0.0f;
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 128 + 16 * NT * wave + 16 * nt + n;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      if (a.splits == 1) store_out4(a, t, hq, 16 * d + 4 * g, o[nt][d], m[nt], l[nt]);
+      if (a.splits == 1) store_out4(a, t, hq, 16 * d + 4 * g, o[nt][d], m[nt], l[nt], sink);
       else *reinterpret_cast<f32x4*>(a.ws_o + at * D + 16 * d + 4 * g) = o[nt][d];
     }
     if (g == 0) {
@@ -692,12 +695,10 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a, int slo
   const int64_t t = row / a.heads;
   const int hq = static_cast<int>(row - t * a.heads);
   if (t >= a.num_tokens) return;
-  if (LIST) {
-    if (a.req_ids[t] < 0 || a.req_ids[t] >= a.num_seqs) return;
-  } else {
-    if (t < a.qsl[0] || t >= a.qsl[a.num_seqs]) return;
-  }
   const int2 info = a.ws_rows[row];
+  const float sink = a.sinks ? a.sinks[hq] : 0.0f;
+  const int lo = LIST ? a.req_ids[t] : a.qsl[0], hi = LIST ? a.num_seqs : a.qsl[a.num_seqs];
+  if (LIST ? lo < 0 || lo >= hi : t < lo || t >= hi) return;
   const int parts = info.y & 255, at = info.y >> 8;
   // whole already; and a row that no workgroup took (more of them than the call said) names no part
   if (parts < 2 || parts > kMaxSplits || at < 0 || at >= slot_rows || info.x < 0 ||
@@ -726,7 +727,7 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a, int slo
 #pragma unroll
     for (int i = 0; i < 8; ++i) y += lane_value(f, s0 + i) * part[i];
   }
-  if (4 * lane < D) store_out4(a, t, hq, c, y, top, sum);
+  if (4 * lane < D) store_out4(a, t, hq, c, y, top, sum, sink);
   if (lane == 0) store_lse(a, t, hq, top, sum);
 }
 

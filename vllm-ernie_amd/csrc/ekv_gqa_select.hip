@@ -51,9 +51,9 @@ __device__ __forceinline__ void load_q8(const uint16_t* p, bool aligned, float (
   }
 }
 
-// One workgroup per (token, kv head).  Wave w holds the keys of the KPT * 64
-// pages from w * KPT * 64 on, one page a lane and chunk of 64; the n-th largest
-// key comes from three rounds of a histogram, and the chosen pages are written
+// One workgroup per (token, kv head).  Its waves share the pages in order, each
+// with the keys of up to KPT chunks of 64, one page a lane; the n-th largest key
+// comes from three rounds of a histogram, and the chosen pages are written
 // in order by counts of the chunks before.
 template <int D, int WAVES, int KPT>
 __global__ void __launch_bounds__(64 * WAVES) gqa_block_select_kernel(GqaSelectArgs a) {
@@ -87,7 +87,8 @@ __global__ void __launch_bounds__(64 * WAVES) gqa_block_select_kernel(GqaSelectA
 
   // the wave's pages, asked for before anything waits
   const int32_t* bt = a.block_table + b * a.bt_stride;
-  const int base = wave * KPT * 64;
+  const int each = min((a.max_blocks + 64 * WAVES - 1) / (64 * WAVES), KPT);  // chunks of a wave
+  const int base = wave * each * 64;
   auto page_of = [&](int c, int end) {
     const int lp = base + 64 * c + lane;
     return lp < end ? bt[lp] : -1;
@@ -95,11 +96,11 @@ __global__ void __launch_bounds__(64 * WAVES) gqa_block_select_kernel(GqaSelectA
   int page[kAhead ? KPT : 1];
   if constexpr (kAhead) {
 #pragma unroll
-    for (int c = 0; c < KPT; ++c) page[c] = page_of(c, min(a.max_blocks, a.bt_width));
+    for (int c = 0; c < KPT; ++c) page[c] = c < each ? page_of(c, min(a.max_blocks, a.bt_width)) : -1;
   }
   const int all = pos < 0 ? 0 : static_cast<int>(min(pos / kPageTokens + 1, static_cast<int64_t>(a.bt_width)));
   const int nb = __builtin_amdgcn_readfirstlane(min(all, a.max_blocks));
-  const int chunks = min(max((nb - base + 63) / 64, 0), KPT);  // of this wave
+  const int chunks = min(max((nb - base + 63) / 64, 0), each);  // of this wave
 
   // q's codes: one exponent for the group; heads again where a tile has rows left
   float top = 0.0f;
