@@ -248,3 +248,42 @@ def test_a_row_that_is_not_finite_stays_alone(dev):
         assert torch.all(torch.isnan(out[1, 2])) and torch.all(torch.isnan(out[2, 0]))
         assert torch.allclose(out[~bad].float(), want[0][~bad].float(), rtol=2.0 ** -6, atol=2.0 ** -6)
         assert torch.allclose(lse[~bad], want[1][~bad], rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("D,blocks", [(64, 90), (128, 65), (256, 41)])
+@pytest.mark.parametrize("window,with_sinks", [(0, True), (700, False)])
+def test_units_that_fill_the_chip(dev, D, blocks, window, with_sinks):
+    """Decode rows of more than 128 (row, kv head) pairs: no parts, each wave
+    walks several pages; of ragged sequences, some empty, and of lists."""
+    from ernie_kv import ops
+
+    rng = np.random.default_rng(D + window)
+    KV, H, seqs = 6, 18, 25
+    lens = [int(n) for n in rng.integers(1, 90, seqs)]
+    lens[3], lens[11], lens[24] = blocks * 64 - 5, blocks * 40, blocks * 64
+    rows = [1] * seqs
+    rows[7], rows[20] = 0, 2
+    lens[20] += 1
+    layer = Layer(dev, rng, lens, KV, D, summary=False)
+    q, pos, seq, tq, tpos, tqsl = batch(dev, rng, lens, rows, H, D)
+    sinks = (2 * rng.standard_normal(H)).astype(np.float32) if with_sinks else None
+    st = None if sinks is None else to_dev(sinks, dev)
+    assert ops.gqa_attention_workspace(len(pos), seqs, 2, blocks * 64, H, KV, D, dev, window=window).numel() == 16
+    out, lse = attend(ops, layer, tq, tpos, tqsl, blocks * 64, 2, window, st)
+    check_rows(layer, q, bf16_values(out).astype(np.float64), lse.cpu().numpy(), D ** -0.5, list(enumerate(seq)), sinks,
+               lambda t, h: np.arange(max(0, pos[t] - window + 1) if window else 0, pos[t] + 1))
+
+    # lists of any order with gaps, of the same rows
+    ids = np.stack([[rng.permutation(blocks) for _ in range(KV)] for _ in pos]).astype(np.int32)
+    ids[rng.random(ids.shape) < 0.1] = -1
+    ids[5, 2] = -1
+    o2, l2 = torch.full_like(out, 7.0), torch.full_like(lse, 7.0)
+    assert ops.gqa_block_attention_workspace(len(pos), H, KV, D, blocks, dev).numel() == 16
+    ops.gqa_block_attention(tq, layer.d_cache, KV, layer.d_bt, tpos, to_dev(seq.astype(np.int32), dev), to_dev(ids, dev),
+                            D ** -0.5, o2, l2, sinks=st)
+
+    def seen(t, h):
+        at = (ids[t, h][ids[t, h] >= 0][:, None] * 64 + np.arange(64)).ravel()
+        return at[at <= pos[t]]
+
+    check_rows(layer, q, bf16_values(o2).astype(np.float64), l2.cpu().numpy(), D ** -0.5, list(enumerate(seq)), sinks, seen)

@@ -314,16 +314,20 @@ __device__ __forceinline__ void page_scales(const GqaAttnArgs& a, int h, int dim
 
 // ---------------------------------------------------------------------------
 // Few rows a kv head: one workgroup per (16 NT rows, kv head, range of pages).
-// Each of its 4 waves takes every fourth page of the range through registers,
+// Each of its W waves takes every W-th page of the range through registers,
 // with no LDS in the loop: K as the A operand (16 tokens x 32 channels) against
 // q leaves a lane the scores of one row and of the tokens whose V bytes it
 // loads, so the weights go straight into the product with V.
 // ---------------------------------------------------------------------------
-template <int D, int NT, bool LIST>
-__global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2) gqa_decode_kernel(GqaAttnArgs a) {
+// Waves of a SIMD that the registers allow.
+template <int D, int NT>
+constexpr int kDecodeWaves = NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2;
+
+template <int D, int NT, int W, bool LIST>
+__global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kernel(GqaAttnArgs a) {
   constexpr int S = D / 64, DT = D / 16;
-  __shared__ float so[4][16][D + 4];
-  __shared__ float2 sml[4][16];
+  __shared__ float so[W][16][D + 4];
+  __shared__ float2 sml[W][16];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   GqaPart p;
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
   int pb = p.part * share, pe = LIST ? a.n_ids : dynamic ? p.pages : a.bt_width;
   if (p.part < p.parts - 1) pe = min(pe, pb + share);
   int page, lp;
-  if (early) lp = list(pb + wave + 4 * lane, pe, page);
+  if (early) lp = list(pb + wave + W * lane, pe, page);
 
   // q in registers where they are few, else in LDS (as operand pieces of 64 lanes)
   constexpr bool kQLds = NT * D >= 128;
@@ -419,8 +423,8 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
     for (int d = 0; d < DT; ++d) vr[d] = load16(r, v_at + 1024 * (d & 3), 4096 * (d >> 2));
   };
 
-  for (int p0 = pb + wave; p0 < pe; p0 += 256) {
-    if (!listed || p0 != pb + wave) lp = list(p0 + 4 * lane, pe, page);
+  for (int p0 = pb + wave; p0 < pe; p0 += 64 * W) {
+    if (!listed || p0 != pb + wave) lp = list(p0 + W * lane, pe, page);
     if (page >= a.num_pages || lp * static_cast<int64_t>(kPageTokens) > pmax) page = -1;
     float ks, vs;
     page_scales(a, h, D, page, ks, vs);
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
     }
   }
 
-  // the four waves' parts of each row
+  // the waves' parts of each row
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     l[nt] += __shfl_xor(l[nt], 16, 64);
@@ -492,28 +496,28 @@ __global__ void __launch_bounds__(256, NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2)
     for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&so[wave][n][16 * d + 4 * g]) = o[nt][d];
     if (g == 0) sml[wave][n] = make_float2(m[nt], l[nt]);
     __syncthreads();
-    const int row = tid >> 4, r = r0 + 16 * nt + row;
+    const int row = (tid >> 4) & 15, r = r0 + 16 * nt + row;
     if (r >= rows) continue;
     const int64_t t = t0 + r / a.group;
     const int hq = h * a.group + r % a.group;
     const float sink = a.sinks ? a.sinks[hq] : 0.0f;
-    float top = kNone, sum = 0.0f, f[4];
+    float top = kNone, sum = 0.0f, f[W];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, sml[w][row].x);
+    for (int w = 0; w < W; ++w) top = fmaxf(top, sml[w][row].x);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
       f[w] = __builtin_amdgcn_exp2f(sml[w][row].x - top);
       sum += f[w] * sml[w][row].y;
     }
 #pragma unroll
-    for (int c = 4 * (tid & 15); c < D; c += 64) {
+    for (int c = 4 * (tid & 15) + 64 * (tid >> 8); c < D; c += 16 * W) {
       f32x4 y = {};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) y += f[w] * *reinterpret_cast<const f32x4*>(&so[w][row][c]);
+      for (int w = 0; w < W; ++w) y += f[w] * *reinterpret_cast<const f32x4*>(&so[w][row][c]);
       if (p.parts == 1) store_out4(a, t, hq, c, y, top, sum, sink);
       else *reinterpret_cast<f32x4*>(a.ws_o + (static_cast<int64_t>(blockIdx.x) * (16 * NT) + 16 * nt + row) * D + c) = y;
     }
-    if ((tid & 15) == 0) {
+    if ((tid & 15) == 0 && tid < 256) {
       if (p.parts == 1) store_lse(a, t, hq, top, sum);
       else a.ws_ml[blockIdx.x * (16 * NT) + 16 * nt + row] = make_float2(top, sum);
       if (a.slots && p.part == 0) a.ws_rows[t * a.heads + hq] = make_int2(p.first, p.parts | (16 * nt + row) << 8);
@@ -738,7 +742,7 @@ struct GqaPlan {
   int row_tiles;  // 16-row tiles of a workgroup: 1, 2, 4 in every wave, or 8 over its four waves
   int tiles, splits, split_pages, budget;
   int64_t units, slots;  // slots: workgroups
-  bool join;
+  bool join, wide;
 };
 
 // seqs: sequences (dense) or tokens (selected blocks); rows: query rows a kv
@@ -751,13 +755,28 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int kv_heads, int dim, bool 
   p.tiles = static_cast<int>((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
   p.units = seqs * kv_heads * p.tiles;
   const int64_t pages = std::max<int64_t>(pages_of(std::min<int64_t>(rows, 16 * p.row_tiles)), 1);
+  const int per_simd = p.row_tiles * dim == 64 ? 4 : p.row_tiles * dim == 128 ? 3 : 2;
+  const int wide_waves = 4 * per_simd;
+  if (p.row_tiles == 1 && pages > 4 && p.units <= 256 &&
+      (pages <= wide_waves || (p.units > 128 && pages <= 6 * wide_waves))) {
+    // One workgroup of all the waves that a CU holds to a unit, and no parts to
+    // join, where a wave has one page or where units fill most of the chip.
+    // 8 kv heads of 128, parts and their join against this, in us: 1 sequence
+    // of 8 pages 9.1 and 7.7, of 16 pages 9.2 and 10.3, of 64 pages 10.5 and
+    // 25.7; 64 listed pages of 16 tokens 43 and 47, of 17 tokens 49 and 48, of
+    // 32 tokens 70 and 63 (with their selection); 32 sequences of 500 to 1,000
+    // tokens 20 and 13.5, of 1,500 to 3,000 tokens 41 and 34.
+    p.wide = true;
+    p.splits = 1, p.split_pages = static_cast<int>(pages), p.slots = p.units;
+    return p;
+  }
   // workgroups that run at once
-  const int64_t round = 256 * (p.row_tiles == 8 ? 2 : p.row_tiles * dim == 64 ? 4 : p.row_tiles * dim == 128 ? 3 : 2);
+  const int64_t round = 256 * (p.row_tiles == 8 ? 2 : per_simd);
   if (!list && p.row_tiles < 8 && seqs > 1 && seqs <= 64 && pages > 8) {
     // Sequences of a dense call differ in length: their parts are shared out on
     // the device, one round of the chip, or as many as leave two parts a unit
     // (13 sequences of 2,000 to 48,000 tokens, 8 kv heads of 128: 82 us with
-    // 2,048 equal parts of the longest one, 72 so).
+    // 2,048 equal parts of the longest one, 74 so).
     p.slots = round * std::max<int64_t>((2 * p.units + round - 1) / round, 1);
     p.budget = static_cast<int>(p.slots / (kv_heads * static_cast<int64_t>(p.tiles)));
     p.split_pages = static_cast<int>(std::min<int64_t>(pages, 1 << 30));
@@ -765,7 +784,8 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int kv_heads, int dim, bool 
     p.join = true;
     return p;
   }
-  // One round: 32 rows of 64 listed pages, 8 kv heads: 52 us at 768, 56 at 2,048.
+  // One round of the chip (32 rows of 64 listed pages, 8 kv heads, in parts:
+  // 52 us in 768 workgroups, 56 in 2,048).
   // Pages of a part.  Of many rows: shorter parts where units are fewer than CUs
   // (4 sequences of 4,096 tokens, 16 rows, 8 kv heads of 128: 37 us at 16, 31 at
   // 8), longer ones where each CU has one already (32 of 1,000: 50 us in two
@@ -801,7 +821,7 @@ static int64_t plan_bytes(const GqaPlan& p, int64_t num_tokens, int64_t heads, i
 }
 
 template <int D, bool LIST>
-static int launch_decode(const GqaAttnArgs& a, int row_tiles, int64_t blocks, hipStream_t s) {
+static int launch_decode(const GqaAttnArgs& a, int row_tiles, bool wide, int64_t blocks, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(blocks));
   if constexpr (!LIST) {
     if (row_tiles == 8) {
@@ -812,12 +832,14 @@ static int launch_decode(const GqaAttnArgs& a, int row_tiles, int64_t blocks, hi
       gqa_prefill_kernel<D><<<grid, 64 * PrefillShape<D>::kWaves, kBytes, s>>>(a);
     }
   }
-  if (row_tiles == 1) gqa_decode_kernel<D, 1, LIST><<<grid, 256, 0, s>>>(a);
+  constexpr int kWide = 4 * kDecodeWaves<D, 1>;
+  if (row_tiles == 1 && wide) gqa_decode_kernel<D, 1, kWide, LIST><<<grid, 64 * kWide, 0, s>>>(a);
+  else if (row_tiles == 1) gqa_decode_kernel<D, 1, 4, LIST><<<grid, 256, 0, s>>>(a);
   if constexpr (D <= 128) {
-    if (row_tiles == 2) gqa_decode_kernel<D, 2, LIST><<<grid, 256, 0, s>>>(a);
+    if (row_tiles == 2) gqa_decode_kernel<D, 2, 4, LIST><<<grid, 256, 0, s>>>(a);
   }
   if constexpr (D == 64) {
-    if (row_tiles == 4) gqa_decode_kernel<D, 4, LIST><<<grid, 256, 0, s>>>(a);
+    if (row_tiles == 4) gqa_decode_kernel<D, 4, 4, LIST><<<grid, 256, 0, s>>>(a);
   }
   int rc = ekv_launch_status();
   if (rc || !a.slots) return rc;
@@ -846,9 +868,9 @@ static int launch_attn(GqaAttnArgs& a, const GqaPlan& p, int dim, void* workspac
     a.ws_ml = reinterpret_cast<float2*>(a.ws_o + p.slots * 16 * p.row_tiles * dim);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dim == 64) return launch_decode<64, LIST>(a, p.row_tiles, p.slots, s);
-  if (dim == 128) return launch_decode<128, LIST>(a, p.row_tiles, p.slots, s);
-  return launch_decode<256, LIST>(a, p.row_tiles, p.slots, s);
+  if (dim == 64) return launch_decode<64, LIST>(a, p.row_tiles, p.wide, p.slots, s);
+  if (dim == 128) return launch_decode<128, LIST>(a, p.row_tiles, p.wide, p.slots, s);
+  return launch_decode<256, LIST>(a, p.row_tiles, p.wide, p.slots, s);
 }
 
 static int attn_args(GqaAttnArgs& a, const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride,
