@@ -287,3 +287,29 @@ def test_units_that_fill_the_chip(dev, D, blocks, window, with_sinks):
         return at[at <= pos[t]]
 
     check_rows(layer, q, bf16_values(o2).astype(np.float64), l2.cpu().numpy(), D ** -0.5, list(enumerate(seq)), sinks, seen)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 130])
+def test_a_cache_of_zeros(dev, D, rows):
+    """Pages that nothing was written to, their scales 0 as in a warm-up's
+    cache: scores of 0 over the tokens a row sees, and values of 0."""
+    from ernie_kv import ops
+
+    KV, H, n = 2, 4, 150
+    cache = torch.zeros((3, ops.gqa_page_bytes(KV, D)), dtype=torch.uint8, device=dev)
+    bt = torch.arange(3, dtype=torch.int32, device=dev)[None]
+    pos = torch.arange(n - rows, n, device=dev)
+    q = bf16_tensor(randn_bf16(np.random.default_rng(D), (rows, H, D)), dev)
+    for scale in (0.1, 1e-38):
+        out = torch.full((rows, H, D), 7.0, dtype=torch.bfloat16, device=dev)
+        lse = torch.empty((rows, H), device=dev)
+        ops.gqa_attention(q, cache, KV, bt, pos, to_dev(np.array([0, rows], np.int32), dev), rows, n, scale, out, lse)
+        assert torch.all(out == 0)
+        want = torch.log(pos.double() + 1)[:, None]
+        assert torch.all((lse.double() - want).abs() <= 2.0 ** -20 * want + 2.0 ** -20)  # 32-bit sums of up to 150 ones
+    ids = torch.arange(3, dtype=torch.int32, device=dev).expand(rows, KV, 3)
+    out.fill_(7.0)
+    ops.gqa_block_attention(q, cache, KV, bt, pos, torch.zeros(rows, dtype=torch.int32, device=dev), ids.contiguous(),
+                            0.1, out, lse)
+    assert torch.all(out == 0) and torch.isfinite(lse).all()

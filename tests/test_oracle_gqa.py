@@ -162,6 +162,7 @@ def _norm(**o):
     ("ekv_gqa_attention", _attn(win=-1), 1, "negative"),
     ("ekv_gqa_attention", _attn(scale=0.0), 1, "scale"),
     ("ekv_gqa_block_attention", _blocks(scale=-1.0), 1, "scale"),
+    ("ekv_gqa_attention", _attn(scale=float("inf")), 1, "scale"),
     ("ekv_gqa_attention", _attn(out=X + 2), 1, "8-byte"),
     ("ekv_gqa_attention", _attn(oh=130), 1, "8-byte"),
     ("ekv_gqa_attention", _attn(ml=100_000), 3, "workspace"),

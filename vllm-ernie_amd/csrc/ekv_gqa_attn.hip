@@ -302,13 +302,14 @@ __device__ __forceinline__ void load_q(const GqaAttnArgs& a, const uint16_t* row
 }
 
 // The scales of lane i's page (page < 0: none) for head h, K's with the softmax
-// scale in log2 units.
+// scale in log2 units.  K's stays above zero, as a masked score needs it: the
+// scale of a page that was never written in a cache of zeros is 0.
 __device__ __forceinline__ void page_scales(const GqaAttnArgs& a, int h, int dim, int page, float& ks, float& vs) {
   ks = vs = 0.0f;
   if (page >= 0) {
     const float* sc = reinterpret_cast<const float*>(a.cache + page * a.page_stride +
                                                      2ll * a.kv_heads * kPageTokens * dim) + h;
-    ks = sc[0] * a.scale_log2, vs = sc[a.kv_heads];
+    ks = fmaxf(sc[0] * a.scale_log2, 0x1p-126f), vs = sc[a.kv_heads];
   }
 }
 
@@ -881,7 +882,7 @@ static int attn_args(GqaAttnArgs& a, const uint16_t* q, int64_t q_tok_stride, in
   EKV_CHECK(gqa_dim(dim), "dim must be 64, 128 or 256");
   EKV_CHECK(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "heads must be a multiple of kv_heads");
   EKV_CHECK(num_tokens >= 0 && num_seqs >= 0 && num_pages >= 0 && bt_width >= 0, "negative sizes");
-  EKV_CHECK(scale > 0.0f, "scale must be positive");
+  EKV_CHECK(scale > 0.0f && scale <= 0x1.fffffep127f, "scale must be positive and finite");
   a = GqaAttnArgs{};
   if (!num_tokens || !num_seqs) return kOk;
   EKV_CHECK(q && (cache || !num_pages) && (block_table || !bt_width) && positions && out, "null pointer");
