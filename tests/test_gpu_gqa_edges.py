@@ -313,3 +313,37 @@ def test_a_cache_of_zeros(dev, D, rows):
     ops.gqa_block_attention(q, cache, KV, bt, pos, torch.zeros(rows, dtype=torch.int32, device=dev), ids.contiguous(),
                             0.1, out, lse)
     assert torch.all(out == 0) and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("D,seqs", [(64, 40), (128, 70), (256, 130)])
+def test_a_prompt_among_many_rows(dev, D, seqs):
+    """One long chunk among sequences of single rows, some without any, rows
+    behind the last one: the write's bytes and the attention of every sequence,
+    and the same of a call of up to the bounds' lengths."""
+    from ernie_kv import ops
+
+    rng = np.random.default_rng(seqs)
+    KV, H = 1, 8
+    rows = [int(r) for r in rng.integers(0, 3, seqs)]
+    rows[0], rows[seqs // 2], rows[-1] = 0, 700, 1
+    ctx = [int(n) for n in rng.integers(0, 100, seqs)]
+    layer = Layer(dev, rng, ctx, KV, D, extra=700)
+    k, v, pos, qsl = layer.step(rows)
+    T = len(pos)
+    pad = [np.concatenate([x, np.ones((5,) + x.shape[1:], x.dtype)]) for x in (k, v)]
+    tpos = np.concatenate([pos, np.zeros(5, np.int64)])
+    gqa.append(k, v, pos, qsl, layer.bt, layer.cache, layer.summary)
+    for bound in (700, 8192):
+        c, s = layer.d_cache.clone(), layer.d_summary.clone()
+        ops.gqa_append(*(bf16_tensor(x, dev) for x in pad), to_dev(tpos, dev), to_dev(qsl, dev), bound, layer.d_bt, c, s)
+        assert np.array_equal(c.cpu().numpy(), layer.cache) and np.array_equal(s.cpu().numpy(), layer.summary)
+    layer.d_cache = c
+    q = randn_bf16(rng, (T + 5, H, D))
+    out, lse = attend(ops, layer, bf16_tensor(q, dev), to_dev(tpos, dev), to_dev(qsl, dev), 800, 700)
+    assert torch.all(out[T:] == 7) and torch.all(lse[T:] == 7)
+    seq = np.repeat(np.arange(seqs), rows)
+    some = sorted(set(np.nonzero(seq != seqs // 2)[0]) | set(T // 2 + rng.integers(-340, 340, 30)) | {0, T - 1})
+    check_rows(layer, q, bf16_values(out).astype(np.float64), lse.cpu().numpy(), D ** -0.5, [(t, seq[t]) for t in some],
+               None, lambda t, h: np.arange(pos[t] + 1))
+    again = attend(ops, layer, bf16_tensor(q, dev), to_dev(tpos, dev), to_dev(qsl, dev), 800, 8192)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])

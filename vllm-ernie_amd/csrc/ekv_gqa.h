@@ -47,6 +47,31 @@ __device__ __forceinline__ int pow2_exponent(float amax, float inv_top) {
 constexpr float kInv448 = 0x1.24924ap-9f;  // fl32(1 / 448)
 constexpr float kInv127 = 0x1.020408p-7f;  // fl32(1 / 127)
 
+// Slots (pages to write, tiles of rows) of a call's sequences, one sequence's
+// behind the other's: at(token, b) is the first slot of sequence b, whose tokens
+// begin at `token`.  Returns the sequence of a slot, `in` its slot among them;
+// -1 where there is none.  Each step narrows it down 64 times; offsets that do
+// not ascend give some sequence.
+template <typename At>
+__device__ __forceinline__ int slot_seq(const int32_t* qsl, int num_seqs, int num_tokens, int slot, At at, int& in) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  int b = 0, step = 1;
+  while (64 * step < num_seqs) step *= 64;
+  while (true) {
+    const int mine = b + step * lane;
+    const int first = mine < num_seqs ? at(min(max(qsl[mine], 0), num_tokens), mine) : 0x7fffffff;
+    const uint64_t upto = __ballot(first <= slot);
+    if (!upto) return -1;
+    const int last = 63 - __builtin_clzll(upto);
+    b += step * last;
+    if (step == 1) {
+      in = slot - __builtin_amdgcn_readlane(first, last);
+      return b;
+    }
+    step >>= 6;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // RMS norm of a head and the rotation of a slice of its channels.  A row of D
 // channels is held by LPR lanes (a power of two, at least D / 8), 8 channels
