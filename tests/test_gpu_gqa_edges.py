@@ -347,3 +347,26 @@ def test_a_prompt_among_many_rows(dev, D, seqs):
                None, lambda t, h: np.arange(pos[t] + 1))
     again = attend(ops, layer, bf16_tensor(q, dev), to_dev(tpos, dev), to_dev(qsl, dev), 800, 8192)
     assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+@pytest.mark.parametrize("seqs,spike", [(64, 9000), (100, 0), (100, 9000), (256, 0), (256, 9000), (257, 9000)])
+def test_sequences_of_like_and_unlike_lengths(dev, seqs, spike):
+    """Decode rows whose sequences are nearly equal (one part each), or one of
+    them long (shared out by pages), at both ends of what is shared out."""
+    from ernie_kv import ops
+
+    rng = np.random.default_rng(seqs + spike)
+    lens = [int(n) for n in rng.integers(590, 641, seqs)]
+    if spike:
+        lens = [n - 400 for n in lens]
+        lens[seqs // 3] = spike
+    KV, D, H = 8, 64, 8
+    few = sorted({0, seqs // 3, seqs - 1} | set(int(b) for b in rng.integers(0, seqs, 9)))
+    layer = Layer(dev, rng, [lens[b] for b in few], KV, D, summary=False)
+    bt = np.zeros((seqs, layer.bt.shape[1]), np.int32)  # the other sequences read pages of the same cache
+    bt[:] = layer.bt[rng.integers(0, len(few), seqs)]
+    bt[few] = layer.bt
+    q, pos, seq, tq, tpos, tqsl = batch(dev, rng, lens, [1] * seqs, H, D)
+    out, lse = attend(ops, layer, tq, tpos, tqsl, max(lens), 1, bt=to_dev(bt, dev))
+    check_rows(layer, q, bf16_values(out).astype(np.float64), lse.cpu().numpy(), D ** -0.5,
+               [(b, i) for i, b in enumerate(few)], None, lambda t, h: np.arange(pos[t] + 1))

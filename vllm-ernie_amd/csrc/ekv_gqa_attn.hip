@@ -59,47 +59,84 @@ struct GqaPart {
   int pages;                // of a part (static), or of the unit as far as known (dynamic)
 };
 
-// Which part of what workgroup i takes where up to 64 sequences share the chip
+// Which part of what workgroup i takes where up to 64 M sequences share the chip
 // by their lengths: every workgroup finds the same smallest Q at which parts of
 // Q pages fit the budget.  A sequence's length is taken from its last row, which
-// decides the shares only.
+// decides the shares only.  Lane i holds the sequences M i .. M i + M - 1.
+template <int M>
 __device__ __forceinline__ bool find_part(const GqaAttnArgs& a, int i, GqaPart& p) {
   const int lane = static_cast<int>(threadIdx.x) & 63, per = a.kv_heads * a.tiles;
-  int w = 0;
-  if (lane < a.num_seqs) {
-    const int t0 = a.qsl[lane], t1 = min(a.qsl[lane + 1], a.num_tokens);
+  int w[M];
+#pragma unroll
+  for (int k = 0; k < M; ++k) {
+    const int b = M * lane + k;
+    w[k] = 0;
+    if (b >= a.num_seqs) continue;
+    const int t0 = a.qsl[b], t1 = min(a.qsl[b + 1], a.num_tokens);
     if (t0 >= 0 && t1 > t0) {
       const int64_t pos = a.positions[t1 - 1];
-      w = static_cast<int>(min(max(pos, static_cast<int64_t>(0)) / kPageTokens + 1, static_cast<int64_t>(max(a.bt_width, 1))));
-      if (a.window) w = min(w, a.split_pages);  // the most pages a tile sees
+      w[k] = static_cast<int>(min(max(pos, static_cast<int64_t>(0)) / kPageTokens + 1, static_cast<int64_t>(max(a.bt_width, 1))));
+      if (a.window) w[k] = min(w[k], a.split_pages);  // the most pages a tile sees
     }
   }
-  auto sum = [](int v) {
+  auto sum = [](const int (&v)[M]) {
+    int x = v[0];
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
-    return __builtin_amdgcn_readfirstlane(v);
+    for (int k = 1; k < M; ++k) x += v[k];
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, 64);
+    return __builtin_amdgcn_readfirstlane(x);
   };
-  int q = max((sum(w) + a.budget - 1) / a.budget, 4), mine;
+  const int all = sum(w);
+  int q = max((all + a.budget - 1) / a.budget, 4), mine[M];
+  if (M > 1) {
+    // Nearly equal lengths of sequences that fill a round of the chip by
+    // themselves (a budget of two parts each, rounded up) stay whole: 96 of
+    // 8,192 tokens, 8 kv heads of 128: 293 -> 283 us, 266 in a grid of equal
+    // parts.
+    int longest = w[0], some[M];
+#pragma unroll
+    for (int k = 0; k < M; ++k) longest = max(longest, w[k]), some[k] = w[k] > 0;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) longest = max(longest, __shfl_xor(longest, m, 64));
+    const int count = sum(some);
+    if (4ll * longest * count <= 5ll * all && 2 * a.budget < 5 * count) q = max(q, longest);
+  }
   while (true) {
-    mine = w ? min(max(static_cast<int>(ceilf(static_cast<float>(w) * (1.0f / static_cast<float>(q)))), 1), 64) : 0;
+    const float inv = 1.0f / static_cast<float>(q);
+#pragma unroll
+    for (int k = 0; k < M; ++k)
+      mine[k] = w[k] ? min(max(static_cast<int>(ceilf(static_cast<float>(w[k]) * inv)), 1), kMaxSplits) : 0;
     if (sum(mine) <= a.budget) break;  // reached: from the longest sequence on there is one part each
     q += (q >> 4) + 1;
   }
-  int upto = mine;
+  int own = mine[0];
+#pragma unroll
+  for (int k = 1; k < M; ++k) own += mine[k];
+  int upto = own;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
     const int x = __shfl_up(upto, m, 64);
     if (lane >= m) upto += x;
   }
   const int j = i / per, ht = i - j * per;
-  const uint64_t at = __ballot(j < upto && j >= upto - mine);
+  const uint64_t at = __ballot(j < upto && j >= upto - own);
   if (!at) return false;
-  p.seq = __builtin_ctzll(at);
-  p.h = ht % a.kv_heads, p.tile = ht / a.kv_heads;
-  p.parts = __builtin_amdgcn_readlane(mine, p.seq);
-  const int before = __builtin_amdgcn_readlane(upto, p.seq) - p.parts;
-  p.part = j - before, p.first = before * per + ht, p.pages = __builtin_amdgcn_readlane(w, p.seq);
-  return true;
+  const int holder = __builtin_ctzll(at);
+  int before = __builtin_amdgcn_readlane(upto - own, holder);
+#pragma unroll
+  for (int k = 0; k < M; ++k) {
+    const int parts = __builtin_amdgcn_readlane(mine[k], holder);
+    if (j < before + parts) {
+      p.seq = M * holder + k;
+      p.h = ht % a.kv_heads, p.tile = ht / a.kv_heads;
+      p.parts = parts, p.part = j - before, p.first = before * per + ht;
+      p.pages = __builtin_amdgcn_readlane(w[k], holder);
+      return true;
+    }
+    before += parts;
+  }
+  return false;
 }
 
 // 8 e4m3fn codes times a power of two -> bf16.
@@ -335,7 +372,8 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
   GqaPart p;
   const bool dynamic = !LIST && a.budget;
   if (dynamic) {
-    if (!find_part(a, static_cast<int>(blockIdx.x), p)) return;
+    if (!(a.num_seqs <= 64 ? find_part<1>(a, static_cast<int>(blockIdx.x), p) : find_part<4>(a, static_cast<int>(blockIdx.x), p)))
+      return;
   } else {
     const int unit = static_cast<int>(blockIdx.x) % a.units;
     p.h = unit % a.kv_heads, p.tile = unit / a.kv_heads % a.tiles, p.seq = unit / a.kv_heads / a.tiles;
@@ -790,11 +828,12 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int64_t all_rows, int kv_hea
   }
   // workgroups that run at once
   const int64_t round = 256 * (p.row_tiles == 8 ? 2 : per_simd);
-  if (!list && p.row_tiles < 8 && seqs > 1 && seqs <= 64 && pages > 8) {
+  if (!list && p.row_tiles < 8 && seqs > 1 && seqs <= 256 && pages > 8) {
     // Sequences of a dense call differ in length: their parts are shared out on
     // the device, one round of the chip, or as many as leave two parts a unit
     // (13 sequences of 2,000 to 48,000 tokens, 8 kv heads of 128: 82 us with
-    // 2,048 equal parts of the longest one, 74 so).
+    // 2,048 equal parts of the longest one, 74 so; 128 of 500 to 32,768 tokens:
+    // 482 and 385; 95 of 1,000 and one of 65,536: 411 and 74).
     p.slots = round * std::max<int64_t>((2 * p.units + round - 1) / round, 1);
     p.budget = static_cast<int>(p.slots / (kv_heads * static_cast<int64_t>(p.tiles)));
     p.split_pages = static_cast<int>(std::min<int64_t>(pages, 1 << 30));

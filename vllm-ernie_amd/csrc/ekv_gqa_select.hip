@@ -313,7 +313,7 @@ extern "C" int ekv_gqa_block_select(const uint16_t* q, int64_t q_tok_stride, int
             "summary_stride must be a multiple of 16 of at least kv_heads * (dim + 4) bytes");
   EKV_CHECK(num_pages < (int64_t{1} << 31), "too many pages");
   const int64_t grid = static_cast<int64_t>(num_tokens) * kv_heads;
-  EKV_CHECK(grid < (int64_t{1} << 31), "too many rows for one call");
+  EKV_CHECK(grid < (1 << 22), "too many rows for one call");  // fewer than 2^32 lanes
   GqaSelectArgs a{};
   a.q = q, a.q_tok_stride = q_tok_stride, a.q_head_stride = q_head_stride;
   a.q_aligned = aligned16(q) && q_tok_stride % 8 == 0 && q_head_stride % 8 == 0;
