@@ -303,6 +303,7 @@ __device__ void gqa_append_block(const GqaAppendArgs& a, int block) {
     for (int t = 0; t < 4; ++t) {
       const int r = 16 * t + 4 * g + i;
       const bool have = r >= first && r < end;
+      if (!__any(have)) continue;  // one token's row is one wave's: 64 tokens, 8 kv heads of 128: 10.9 -> 8.6 us
       float v[E][8];
 #pragma unroll
       for (int e = 0; e < E; ++e) unpack_bf16x8(kx[t][e], v[e]);
