@@ -191,7 +191,7 @@ struct RowRange {
 // kscale > 0 takes a raw score to log2 units.  A reference is a maximum that the
 // row has had, and moves only where the page's weights around it grow past
 // kMoveAt.  kBySum sees that in their sums, which costs no maximum but the raw
-// scores' registers (many rows: the products bound the kernel; 2,009 -> 1,950 us
+// scores' registers (many rows, where the products bound the kernel: 3% less time
 // at 4,096 rows); else in the largest score.  Masks are selects without branches.
 template <bool kBySum, int NT, int DT>
 __device__ __forceinline__ void softmax_page(f32x4 (&x)[NT][4], float kscale, bool whole, int first, int g,
@@ -356,7 +356,15 @@ __device__ __forceinline__ void page_scales(const GqaAttnArgs& a, int h, int dim
 // Each of its W waves takes every W-th page of the range through registers,
 // with no LDS in the loop: K as the A operand (16 tokens x 32 channels) against
 // q leaves a lane the scores of one row and of the tokens whose V bytes it
-// loads, so the weights go straight into the product with V.
+// loads, so the weights go straight into the product with V.  The next page's K
+// and V are asked for as soon as the products that read their registers are
+// issued.
+//
+// Bound by the read of the pages (32 rows of 64 heads at 131,072 tokens, 8 kv
+// heads of 128: 8.6 GB in 1,412 us, 6.1 TB/s; 13 sequences of 2,000 to 48,000:
+// 384 MB in 74 us, 5.2 TB/s); listed pages that rows share by their caches (333
+// rows of 32 blocks, 4 kv heads: 698 MB in 73 us, 9.6 TB/s); a short context by
+// one page's chain of reads (4,096 tokens: 6.5 us).
 // ---------------------------------------------------------------------------
 // Waves of a SIMD that the registers allow.
 template <int D, int NT>
@@ -570,8 +578,15 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
 // Its waves (4 of 32 rows; 8 of 16 at 256 channels, whose sums of 32 would leave
 // one wave a SIMD: 1,490 -> 1,100 us at 2,048 rows) share every page: each brings
 // its part of it, converted to bf16 once, into LDS in the order of the operands
-// (1 KB reads of 64 consecutive 16-byte pieces), while the page before is
-// multiplied.
+// (1 KB reads of 64 consecutive 16-byte pieces, no bank conflicts), while the
+// page before is multiplied.
+//
+// Bound by the matrix cores and the weights' exponentials, which two waves a
+// SIMD overlap in part (4,096 rows of 32 heads of 128 at 32,768 tokens: 1,776 to
+// 1,860 us, 1,110 to 1,160 TFLOP/s, matrix cores busy 46% of the cycles; a
+// product of 8,192^3 reaches 1,128 on the same card, of 16,384^3 1,350).  At 64
+// channels the exponentials are half of the work (2,048 rows at 16,384: 690
+// TFLOP/s), at 256 there are more conversions a product (940).
 // ---------------------------------------------------------------------------
 template <int D>
 struct PrefillShape {
@@ -738,7 +753,9 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
   }
 }
 
-// Joins a row's parts: one wave per (token, head), lane s the s-th part's weight.
+// Joins a row's parts: out = sum_p e^(m_p - m) o_p / sum_p e^(m_p - m) l_p, one
+// wave per (token, head), lane s the s-th part's weight.  Bound by its launch and
+// two trips to memory (4 to 6 us).
 template <int D, bool LIST>
 __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a, int slot_rows) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
@@ -799,7 +816,12 @@ template <typename Pages>
 static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int64_t all_rows, int kv_heads, int dim, bool list, Pages pages_of) {
   GqaPlan p{};
   const int most = dim == 256 ? 1 : dim == 128 ? 2 : 4;
-  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : rows <= (dim == 256 ? 48 : 64) || list ? most : 8;
+  // The kernel of few rows streams a page once for 16 row_tiles rows, what the
+  // registers hold; the one of many rows from there on, in us: 16 sequences of
+  // 16,384 tokens, 8 kv heads, 64 rows of 64 channels 62 and 97, of 128 channels
+  // 140 and 145 (1 of 32,768: 28 and 35); at 72 rows of 128 184 and 149; at 256
+  // channels 32 rows 262 and 268 (1 of 32,768: 37 and 53), 40 rows 331 and 272.
+  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? std::min(2, most) : rows <= (dim == 256 ? 32 : 64) || list ? most : 8;
   p.tiles = static_cast<int>((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
   p.units = seqs * kv_heads * p.tiles;
   // Many sequences of unlike lengths: the tiles that their rows may need, not
