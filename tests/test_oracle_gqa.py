@@ -181,6 +181,18 @@ def test_refusals(lib, name, args, status, message):
 
 
 @pytest.mark.parametrize("name,args", [
+    ("ekv_qk_norm_rope", _norm(T=(1 << 31) - 1)), ("ekv_gqa_append", _append(T=1 << 26, B=1 << 20, mq=64)),
+    ("ekv_gqa_append", _append(T=1 << 26, B=1 << 20, mq=8192)), ("ekv_gqa_attention", _attn(T=1 << 24, B=1 << 24, mq=1)),
+    ("ekv_gqa_attention", _attn(T=(1 << 31) - 1, B=2, mq=(1 << 31) - 1)), ("ekv_gqa_block_select", _select(T=1 << 20)),
+    ("ekv_gqa_block_attention", _blocks(T=1 << 24)),
+])
+def test_grids_past_the_limit(lib, name, args):
+    """A grid holds fewer than 2^32 lanes: larger calls are refused, not cut off."""
+    assert getattr(lib, name)(*args) == 1
+    assert "too many rows" in lib.ekv_last_error().decode()
+
+
+@pytest.mark.parametrize("name,args", [
     ("ekv_qk_norm_rope", _norm(T=0)), ("ekv_gqa_append", _append(T=0)), ("ekv_gqa_append", _append(B=0)),
     ("ekv_gqa_append", _append(mq=0)), ("ekv_gqa_attention", _attn(T=0)), ("ekv_gqa_attention", _attn(B=0)),
     ("ekv_gqa_attention", _attn(mq=0)), ("ekv_gqa_block_select", _select(n=0, kf=0, kl=0)),
