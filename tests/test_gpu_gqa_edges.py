@@ -370,3 +370,26 @@ def test_sequences_of_like_and_unlike_lengths(dev, seqs, spike):
     out, lse = attend(ops, layer, tq, tpos, tqsl, max(lens), 1, bt=to_dev(bt, dev))
     check_rows(layer, q, bf16_values(out).astype(np.float64), lse.cpu().numpy(), D ** -0.5,
                [(b, i) for i, b in enumerate(few)], None, lambda t, h: np.arange(pos[t] + 1))
+
+
+@pytest.mark.parametrize("D,window", [(64, 0), (128, 0), (128, 900), (128, 8700), (256, 0)])
+def test_long_single_rows_beside_a_chunk(dev, D, window):
+    """Single rows far behind a chunk of the same call, in parts each; the
+    workspace holds what an earlier call might have left there."""
+    from ernie_kv import ops
+
+    rng = np.random.default_rng(D + window)
+    KV, H = 1, 8
+    rows = [1, 2, 300, 0, 1, 3, 1, 1, 2, 1]
+    lens = [9000, 700, 900, 40, 1, 2000, 66, 3000, 129, 17]
+    layer = Layer(dev, rng, lens, KV, D, summary=False)
+    q, pos, seq, tq, tpos, tqsl = batch(dev, rng, lens, rows, H, D)
+    sinks = rng.standard_normal(H).astype(np.float32)
+    n = ops.gqa_attention_workspace(len(pos), len(rows), 300, 9000, H, KV, D, dev, window=window).numel()
+    assert n > 16
+    some = sorted(set(np.nonzero(seq != 2)[0]) | {3 + int(i) for i in rng.integers(0, 300, 25)} | {3, 302})
+    for left in (2, 1 << 16 | 3, -1):
+        ws = torch.full((n // 4 + 1,), left, dtype=torch.int32, device=dev).view(torch.uint8)
+        out, lse = attend(ops, layer, tq, tpos, tqsl, 9000, 300, window, to_dev(sinks, dev), workspace=ws)
+        check_rows(layer, q, bf16_values(out).astype(np.float64), lse.cpu().numpy(), D ** -0.5, [(t, seq[t]) for t in some],
+                   sinks, lambda t, h: np.arange(max(0, pos[t] - window + 1) if window else 0, pos[t] + 1))

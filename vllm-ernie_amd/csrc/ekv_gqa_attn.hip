@@ -47,7 +47,10 @@ struct GqaAttnArgs {
   int32_t by_rows;          // 1: many rows, `tiles` in all, a sequence's after those of the one before
   int32_t budget;           // 0, or the parts of a (kv head, tile) that its sequences share
   int32_t slots, part_step; // workgroups, and how far apart those of a unit are
-  int2* ws_rows;            // [T, heads]: first workgroup, parts | row of its tile << 8
+  // 0, or of a call that both kernels share: sequences of up to `few` rows are the
+  // one's of few rows (kind 0), the others the one's of many (kind 1)
+  int32_t few, kind;
+  int2* ws_rows;            // [T, heads]: first workgroup, parts | row of its tile << 8 | kind << 16
   float2* ws_ml;            // [slots, rows]: (reference in log2 units, sum)
   float* ws_o;              // [slots, rows, D]
 };
@@ -73,7 +76,7 @@ __device__ __forceinline__ bool find_part(const GqaAttnArgs& a, int i, GqaPart& 
     w[k] = 0;
     if (b >= a.num_seqs) continue;
     const int t0 = a.qsl[b], t1 = min(a.qsl[b + 1], a.num_tokens);
-    if (t0 >= 0 && t1 > t0) {
+    if (t0 >= 0 && t1 > t0 && (!a.few || (t1 - t0) * a.group <= a.few)) {
       const int64_t pos = a.positions[t1 - 1];
       w[k] = static_cast<int>(min(max(pos, static_cast<int64_t>(0)) / kPageTokens + 1, static_cast<int64_t>(max(a.bt_width, 1))));
       if (a.window) w[k] = min(w[k], a.split_pages);  // the most pages a tile sees
@@ -397,7 +400,7 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
   } else {
     b = seq, t0 = a.qsl[b];
     rows = (min(a.qsl[b + 1], a.num_tokens) - t0) * a.group;
-    if (t0 < 0) return;
+    if (t0 < 0 || (a.few && rows > a.few)) return;
   }
   const int r0 = p.tile * 16 * NT;
   if (r0 >= rows) return;
@@ -568,7 +571,8 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
     if ((tid & 15) == 0 && tid < 256) {
       if (p.parts == 1) store_lse(a, t, hq, top, sum);
       else a.ws_ml[blockIdx.x * (16 * NT) + 16 * nt + row] = make_float2(top, sum);
-      if (a.slots && p.part == 0) a.ws_rows[t * a.heads + hq] = make_int2(p.first, p.parts | (16 * nt + row) << 8);
+      if (a.ws_rows && p.part == 0)
+        a.ws_rows[t * a.heads + hq] = make_int2(p.first, p.parts | (16 * nt + row) << 8 | a.kind << 16);
     }
   }
 }
@@ -585,7 +589,7 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
 // SIMD overlap in part (4,096 rows of 32 heads of 128 at 32,768 tokens: 1,776 to
 // 1,860 us, 1,110 to 1,160 TFLOP/s, matrix cores busy 46% of the cycles; a
 // product of 8,192^3 reaches 1,128 on the same card, of 16,384^3 1,350).  At 64
-// channels the exponentials are half of the work (2,048 rows at 16,384: 690
+// channels the exponentials are half of the work (2,048 rows at 16,384: 780
 // TFLOP/s), at 256 there are more conversions a product (940).
 // ---------------------------------------------------------------------------
 template <int D>
@@ -615,7 +619,7 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
   }
   const int t0 = a.qsl[b];
   const int rows = (min(a.qsl[b + 1], a.num_tokens) - t0) * a.group;
-  if (t0 < 0 || tile * 128 >= rows) return;
+  if (t0 < 0 || tile * 128 >= rows || (a.few && rows <= a.few)) return;
   const int r0 = tile * 128 + 16 * NT * wave;
   RowRange<NT> rr;
   bf16x8 q[NT][2 * S];
@@ -748,7 +752,8 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
     if (g == 0) {
       if (a.splits == 1) store_lse(a, t, hq, m[nt], l[nt]);
       else a.ws_ml[at] = make_float2(m[nt], l[nt]);
-      if (a.slots && split == 0) a.ws_rows[t * a.heads + hq] = make_int2(unit, a.splits | (16 * (NT * wave + nt) + n) << 8);
+      if (a.ws_rows && split == 0)
+        a.ws_rows[t * a.heads + hq] = make_int2(unit, a.splits | (16 * (NT * wave + nt) + n) << 8 | a.kind << 16);
     }
   }
 }
@@ -767,9 +772,9 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a, int slo
   const float sink = a.sinks ? a.sinks[hq] : 0.0f;
   const int lo = LIST ? a.req_ids[t] : a.qsl[0], hi = LIST ? a.num_seqs : a.qsl[a.num_seqs];
   if (LIST ? lo < 0 || lo >= hi : t < lo || t >= hi) return;
-  const int parts = info.y & 255, at = info.y >> 8;
-  // whole already; and a row that no workgroup took (more of them than the call said) names no part
-  if (parts < 2 || parts > kMaxSplits || at < 0 || at >= slot_rows || info.x < 0 ||
+  const int parts = info.y & 255, at = (info.y >> 8) & 255;
+  // whole already, or the other kernel's; and a row that no workgroup took (more of them than the call said) names no part
+  if (parts < 2 || info.y >> 16 != a.kind || parts > kMaxSplits || at >= slot_rows || info.x < 0 ||
       info.x + static_cast<int64_t>(parts - 1) * a.part_step >= a.slots)
     return;
   const int64_t first = static_cast<int64_t>(info.x) * slot_rows + at, step = static_cast<int64_t>(a.part_step) * slot_rows;
@@ -880,23 +885,48 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int64_t all_rows, int kv_hea
   return p;
 }
 
-static GqaPlan dense_plan(int64_t tokens, int64_t seqs, int64_t max_rows, int group, int kv_heads, int dim,
-                          int64_t max_len, int64_t window) {
-  return gqa_plan(seqs, max_rows * group, tokens * group, kv_heads, dim, false, [&](int64_t rows) {
+// A call's launches: `all`, or where chunks may stand beside single rows that see
+// many pages, the kernel of few rows, in parts, for sequences of up to kFewRows
+// and `all` for the others.  64 heads, 8 kv heads of 128, `all` against both, in
+// us: 8 rows at 131,072 tokens and a chunk of 512 1,433 and 441, 32 at 8,192 and
+// 2,048 371 and 331; at shorter contexts the second launch costs more than it
+// gives: 64 at 2,000 and 4,096 560 and 610, 8 at 1,000 and 1,024 101 and 121.
+struct GqaPlans {
+  GqaPlan all, few;
+  bool both;
+};
+constexpr int kFewRows = 16;
+
+static GqaPlans dense_plans(int64_t tokens, int64_t seqs, int64_t max_rows, int group, int kv_heads, int dim,
+                            int64_t max_len, int64_t window) {
+  auto pages = [&](int64_t rows) {
     const int64_t all = (max_len + kPageTokens - 1) / kPageTokens;
     const int64_t tokens = (rows + group - 1) / group + 1;  // of a tile that begins inside one
     return window ? std::min(all, (window + tokens - 2) / kPageTokens + 2) : all;
-  });
+  };
+  GqaPlans p{};
+  p.all = gqa_plan(seqs, max_rows * group, tokens * group, kv_heads, dim, false, pages);
+  p.both = p.all.by_rows && group <= kFewRows && pages(kFewRows) >= 128;
+  if (p.both) p.few = gqa_plan(seqs, kFewRows, tokens * group, kv_heads, dim, false, pages);
+  return p;
 }
 
-static GqaPlan block_plan(int64_t num_tokens, int group, int kv_heads, int dim, int64_t num_blocks) {
-  return gqa_plan(num_tokens, group, num_tokens * group, kv_heads, dim, true, [&](int64_t) { return num_blocks; });
+static GqaPlans block_plans(int64_t num_tokens, int group, int kv_heads, int dim, int64_t num_blocks) {
+  GqaPlans p{};
+  p.all = gqa_plan(num_tokens, group, num_tokens * group, kv_heads, dim, true, [&](int64_t) { return num_blocks; });
+  return p;
 }
 
 static int64_t rows_bytes(int64_t num_tokens, int64_t heads) { return (num_tokens * heads * 8 + 15) / 16 * 16; }
 
-static int64_t plan_bytes(const GqaPlan& p, int64_t num_tokens, int64_t heads, int64_t dim) {
-  return p.join ? rows_bytes(num_tokens, heads) + p.slots * 16 * p.row_tiles * (dim + 2) * 4 : 0;
+// The parts' sums of a launch.
+static int64_t slots_bytes(const GqaPlan& p, int64_t dim) {
+  return p.join ? p.slots * 16 * p.row_tiles * (dim + 2) * 4 : 0;
+}
+
+static int64_t plan_bytes(const GqaPlans& p, int64_t num_tokens, int64_t heads, int64_t dim) {
+  const int64_t n = slots_bytes(p.all, dim) + (p.both ? slots_bytes(p.few, dim) : 0);
+  return n ? rows_bytes(num_tokens, heads) + n : 0;
 }
 
 template <int D, bool LIST>
@@ -928,30 +958,42 @@ static int launch_decode(const GqaAttnArgs& a, int row_tiles, bool wide, int64_t
 }
 
 template <bool LIST>
-static int launch_attn(GqaAttnArgs& a, const GqaPlan& p, int dim, void* workspace, int64_t workspace_bytes,
+static int launch_attn(GqaAttnArgs& a, const GqaPlans& plans, int dim, void* workspace, int64_t workspace_bytes,
                        void* stream) {
   // grids of fewer than 2^32 lanes
-  EKV_CHECK(p.slots < (1 << 23) && (!p.join || static_cast<int64_t>(a.num_tokens) * a.heads < (1 << 26)),
+  const bool join = plans.all.join || plans.few.join;
+  EKV_CHECK(plans.all.slots < (1 << 23) && plans.few.slots < (1 << 23) &&
+                (!join || static_cast<int64_t>(a.num_tokens) * a.heads < (1 << 26)),
             "too many rows for one call");
-  const int64_t need = plan_bytes(p, a.num_tokens, a.heads, dim);
+  const int64_t need = plan_bytes(plans, a.num_tokens, a.heads, dim);
   if (need > workspace_bytes || (need && !workspace)) {
     set_error("workspace too small");
     return kWorkspaceTooSmall;
   }
   EKV_CHECK(!need || aligned16(workspace), "workspace must be 16-byte aligned");
-  a.tiles = p.tiles, a.units = static_cast<int32_t>(p.units), a.splits = p.splits, a.split_pages = p.split_pages;
-  a.budget = p.budget, a.by_rows = p.by_rows;
-  if (p.join) {
-    a.slots = static_cast<int32_t>(p.slots), a.part_step = p.budget ? a.kv_heads * p.tiles : a.units;
-    uint8_t* const ws = static_cast<uint8_t*>(workspace);
-    a.ws_rows = reinterpret_cast<int2*>(ws);
-    a.ws_o = reinterpret_cast<float*>(ws + rows_bytes(a.num_tokens, a.heads));
-    a.ws_ml = reinterpret_cast<float2*>(a.ws_o + p.slots * 16 * p.row_tiles * dim);
-  }
+  if (need) a.ws_rows = static_cast<int2*>(workspace);
+  uint8_t* sums = static_cast<uint8_t*>(workspace) + rows_bytes(a.num_tokens, a.heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dim == 64) return launch_decode<64, LIST>(a, p.row_tiles, p.wide, p.slots, s);
-  if (dim == 128) return launch_decode<128, LIST>(a, p.row_tiles, p.wide, p.slots, s);
-  return launch_decode<256, LIST>(a, p.row_tiles, p.wide, p.slots, s);
+  auto launch = [&](const GqaPlan& p) {
+    a.tiles = p.tiles, a.units = static_cast<int32_t>(p.units), a.splits = p.splits, a.split_pages = p.split_pages;
+    a.budget = p.budget, a.by_rows = p.by_rows, a.slots = 0;
+    if (p.join) {
+      a.slots = static_cast<int32_t>(p.slots), a.part_step = p.budget ? a.kv_heads * p.tiles : a.units;
+      a.ws_o = reinterpret_cast<float*>(sums);
+      a.ws_ml = reinterpret_cast<float2*>(a.ws_o + p.slots * 16 * p.row_tiles * dim);
+      sums += slots_bytes(p, dim);
+    }
+    if (dim == 64) return launch_decode<64, LIST>(a, p.row_tiles, p.wide, p.slots, s);
+    if (dim == 128) return launch_decode<128, LIST>(a, p.row_tiles, p.wide, p.slots, s);
+    return launch_decode<256, LIST>(a, p.row_tiles, p.wide, p.slots, s);
+  };
+  if (plans.both) {
+    a.few = kFewRows;
+    const int rc = launch(plans.few);
+    if (rc) return rc;
+    a.kind = 1;
+  }
+  return launch(plans.all);
 }
 
 static int attn_args(GqaAttnArgs& a, const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride,
@@ -993,7 +1035,7 @@ extern "C" int64_t ekv_gqa_attention_workspace_size(int32_t num_tokens, int32_t 
       window < 0)
     return 0;
   const int64_t rows = std::min(max_query_len, num_tokens);
-  return plan_bytes(dense_plan(num_tokens, num_seqs, rows, heads / kv_heads, kv_heads, dim, std::max(max_len, 0), window),
+  return plan_bytes(dense_plans(num_tokens, num_seqs, rows, heads / kv_heads, kv_heads, dim, std::max(max_len, 0), window),
                     num_tokens, heads, dim);
 }
 
@@ -1015,14 +1057,14 @@ extern "C" int ekv_gqa_attention(const uint16_t* q, int64_t q_tok_stride, int64_
   EKV_CHECK(qsl, "null pointer");
   a.qsl = qsl, a.window = window;
   const int64_t rows = std::min(max_query_len, num_tokens);
-  return launch_attn<false>(a, dense_plan(num_tokens, num_seqs, rows, a.group, kv_heads, dim, max_len, window), dim,
+  return launch_attn<false>(a, dense_plans(num_tokens, num_seqs, rows, a.group, kv_heads, dim, max_len, window), dim,
                             workspace, workspace_bytes, stream);
 }
 
 extern "C" int64_t ekv_gqa_block_attention_workspace_size(int32_t num_tokens, int32_t heads, int32_t kv_heads,
                                                           int32_t dim, int32_t num_blocks) {
   if (num_tokens <= 0 || kv_heads <= 0 || heads < kv_heads || !gqa_dim(dim)) return 0;
-  return plan_bytes(block_plan(num_tokens, heads / kv_heads, kv_heads, dim, num_blocks), num_tokens, heads, dim);
+  return plan_bytes(block_plans(num_tokens, heads / kv_heads, kv_heads, dim, num_blocks), num_tokens, heads, dim);
 }
 
 extern "C" int ekv_gqa_block_attention(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride,
@@ -1044,6 +1086,6 @@ extern "C" int ekv_gqa_block_attention(const uint16_t* q, int64_t q_tok_stride, 
   EKV_CHECK(req_ids && (blocks || !num_blocks), "null pointer");
   a.req_ids = req_ids, a.ids = blocks, a.ids_tok_stride = blocks_tok_stride, a.ids_head_stride = blocks_head_stride;
   a.n_ids = num_blocks;
-  return launch_attn<true>(a, block_plan(num_tokens, a.group, kv_heads, dim, num_blocks), dim, workspace, workspace_bytes,
+  return launch_attn<true>(a, block_plans(num_tokens, a.group, kv_heads, dim, num_blocks), dim, workspace, workspace_bytes,
                            stream);
 }
