@@ -393,3 +393,69 @@ def test_long_single_rows_beside_a_chunk(dev, D, window):
         out, lse = attend(ops, layer, tq, tpos, tqsl, 9000, 300, window, to_dev(sinks, dev), workspace=ws)
         check_rows(layer, q, bf16_values(out).astype(np.float64), lse.cpu().numpy(), D ** -0.5, [(t, seq[t]) for t in some],
                    sinks, lambda t, h: np.arange(max(0, pos[t] - window + 1) if window else 0, pos[t] + 1))
+
+
+def block_rows(dev, layer, q, pos, req, ids, scale, sinks=None, some=None):
+    """Block attention of rows whose table is ``layer.bt``, checked against the oracle; (out, lse) as they came."""
+    from ernie_kv import ops
+
+    T, H, D = q.shape
+    out = torch.full((T, H, D), 7.0, dtype=torch.bfloat16, device=dev)
+    lse = torch.full((T, H), 7.0, device=dev)
+    bt = layer.d_bt
+    ops.gqa_block_attention(bf16_tensor(q, dev), layer.d_cache, layer.KV, bt, to_dev(pos, dev), to_dev(req, dev),
+                            to_dev(ids, dev), scale, out, lse, sinks=None if sinks is None else to_dev(sinks, dev))
+    known = [(t, req[t]) for t in (range(T) if some is None else some) if 0 <= req[t] < bt.shape[0]]
+    off = [t for t in range(T) if not 0 <= req[t] < bt.shape[0]]
+    assert torch.all(out[off] == 7) and torch.all(lse[off] == 7)
+    pages = layer.bt.shape[1] - 1
+
+    def seen(t, h):
+        j = ids[t, h]
+        at = (j[(j >= 0) & (j < pages)].astype(np.int64)[:, None] * 64 + np.arange(64)).ravel()
+        return at[at <= pos[t]]
+
+    check_rows(layer, q, bf16_values(out).astype(np.float64), lse.cpu().numpy(), scale, known, sinks, seen)
+    return out, lse
+
+
+@pytest.mark.parametrize("D,H,KV", [(64, 12, 4), (128, 16, 2), (128, 16, 16), (128, 16, 8), (256, 32, 8), (256, 10, 2)])
+@pytest.mark.parametrize("n,T", [(5, 70), (24, 131), (33, 260)])
+def test_lists_of_neighbouring_rows(dev, D, H, KV, n, T):
+    """A chunk's rows, whose lists are joined: like and unlike lists, gaps, pages
+    listed again (they count again), pages behind the row or outside the table,
+    rows of no request, and rows of another request between them."""
+    rng = np.random.default_rng(D + n + T)
+    layer = Layer(dev, rng, [64 * 40 - 7, 900], KV, D, summary=False)
+    q = randn_bf16(rng, (T, H, D))
+    pos = np.sort(rng.integers(64 * 20, 64 * 40 - 7, T)).astype(np.int64)
+    req = np.zeros(T, np.int32)
+    ids = np.sort(np.argsort(rng.random((T, KV, 40)), axis=2)[..., :n], axis=2).astype(np.int32)
+    ids[T // 3:T // 2] = ids[T // 3]  # neighbours that agree
+    ids[rng.random(ids.shape) < 0.1] = -1
+    ids[3, 0] = -1
+    ids[8:12, :, 1:3] = ids[8:12, :, :1]  # three mentions
+    ids[20, 0, 0], ids[21, 0, 0] = 1 << 30, -(1 << 31)
+    req[30:33], req[40], req[41], req[T - 2] = 1, -1, 2, 1
+    pos[req == 1] = rng.integers(0, 900, int((req == 1).sum()))
+    pos[50] = -1
+    sinks = rng.standard_normal(H).astype(np.float32)
+    some = sorted(set(range(0, 52, 3)) | {8, 9, 10, 11, 20, 29, 30, 31, 32, 40, 41, 50, T // 3, T // 2 - 1, T - 3, T - 2, T - 1})
+    first = block_rows(dev, layer, q, pos, req, ids, D ** -0.5, sinks, some)
+    again = block_rows(dev, layer, q, pos, req, ids, D ** -0.5, sinks, some[:1])
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_joined_lists_over_long_tables(dev):
+    """Pages past the first 2,048 of a request, which are joined range by range."""
+    rng = np.random.default_rng(77)
+    KV, H, D, T, n, pages = 8, 32, 128, 70, 20, 5000
+    layer = Layer(dev, rng, [64 * 30], KV, D, summary=False)
+    full = layer.bt[0, :30]
+    layer.bt = full[rng.integers(0, 30, (1, pages + 1))].astype(np.int32)
+    layer.d_bt = to_dev(layer.bt, dev)
+    q = randn_bf16(rng, (T, H, D))
+    pos = (64 * pages - 1 - 50 * np.arange(T)[::-1]).astype(np.int64)
+    ids = np.sort(rng.choice(pages, (T, KV, n)), axis=2).astype(np.int32)
+    ids[:, :, :3] = [2047, 2048, 4095]
+    block_rows(dev, layer, q, pos, np.zeros(T, np.int32), ids, 0.1, some=[0, 17, 42, 69])

@@ -35,6 +35,7 @@ struct GqaAttnArgs {
   const int32_t* ids;       // selected blocks: [T, kv_heads, n_ids] logical pages, -1 skipped
   int64_t ids_tok_stride, ids_head_stride;
   int32_t n_ids;
+  int32_t share;            // neighbouring tokens whose lists a workgroup joins
   int32_t window;           // 0: none
   float scale_log2;
   const float* sinks;
@@ -369,19 +370,29 @@ __device__ __forceinline__ void page_scales(const GqaAttnArgs& a, int h, int dim
 // rows of 32 blocks, 4 kv heads: 698 MB in 73 us, 9.6 TB/s); a short context by
 // one page's chain of reads (4,096 tokens: 6.5 us).
 // ---------------------------------------------------------------------------
+// What a workgroup's rows read: all pages, one token's list, or the joined lists
+// of neighbouring tokens.
+enum Pages { kDense, kList, kShared };
+constexpr int kRange = 2048;     // pages that are joined at a time
+constexpr int kShareIds = 256;   // longest lists that are joined
+
 // Waves of a SIMD that the registers allow.
 template <int D, int NT>
 constexpr int kDecodeWaves = NT * D == 64 ? 4 : NT * D == 128 ? 3 : 2;
 
-template <int D, int NT, int W, bool LIST>
+template <int D, int NT, int W, Pages P>
 __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kernel(GqaAttnArgs a) {
   constexpr int S = D / 64, DT = D / 16;
+  constexpr bool LIST = P == kList, SHARE = P == kShared;
+  __shared__ uint32_t row_mask[SHARE ? kRange : 1];  // of a page: the rows that list it
+  __shared__ uint16_t joined[SHARE ? kRange : 1];    // listed pages in order
+  __shared__ int counts[SHARE ? kRange / 64 : 1];
   __shared__ float so[W][16][D + 4];
   __shared__ float2 sml[W][16];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   GqaPart p;
-  const bool dynamic = !LIST && a.budget;
+  const bool dynamic = P == kDense && a.budget;
   if (dynamic) {
     if (!(a.num_seqs <= 64 ? find_part<1>(a, static_cast<int>(blockIdx.x), p) : find_part<4>(a, static_cast<int>(blockIdx.x), p)))
       return;
@@ -397,6 +408,8 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
   if (LIST) {
     t0 = seq, rows = a.group, b = a.req_ids[seq];
     if (b < 0 || b >= a.num_seqs) return;
+  } else if (SHARE) {
+    t0 = seq * a.share, rows = min(a.share, a.num_tokens - t0) * a.group, b = 0;
   } else {
     b = seq, t0 = a.qsl[b];
     rows = (min(a.qsl[b + 1], a.num_tokens) - t0) * a.group;
@@ -409,13 +422,21 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
   // none).  The first ones are asked for before the rows, whose positions and
   // q arrive together with them.
   const int32_t* bt = a.block_table + b * a.bt_stride;
+  int base = 0;          // shared lists: first page of the range
+  uint32_t listing = 0;  // and lane i's page: its row_mask
   auto list = [&](int e, int end, int& page) {
     int lp = -1;
-    if (e < end) lp = LIST ? a.ids[t0 * a.ids_tok_stride + h * a.ids_head_stride + e] : e;
+    if (SHARE) {
+      if (e < end) lp = joined[e];
+      listing = lp >= 0 ? row_mask[lp] : 0;
+      lp += lp >= 0 ? base : 0;
+    } else if (e < end) {
+      lp = LIST ? a.ids[t0 * a.ids_tok_stride + h * a.ids_head_stride + e] : e;
+    }
     page = lp >= 0 && lp < a.bt_width ? bt[lp] : -1;
     return lp;
   };
-  const bool early = LIST || !a.window;
+  const bool early = LIST || (!SHARE && !a.window);
   int share = dynamic ? (p.pages + p.parts - 1) / p.parts : p.pages;
   int pb = p.part * share, pe = LIST ? a.n_ids : dynamic ? p.pages : a.bt_width;
   if (p.part < p.parts - 1) pe = min(pe, pb + share);
@@ -442,7 +463,7 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
   const int pmax = rr.pmax;
   const int low = a.window && pmax >= 0 ? max(rr.pmin - a.window + 1, 0) : 0;  // first token any row sees
   bool listed = early;
-  if (!LIST) {
+  if (P == kDense) {
     const int last = pmax < 0 ? 0 : min(pmax / kPageTokens + 1, a.bt_width), from = low / kPageTokens;
     if (dynamic) {
       listed = early && last == p.pages;
@@ -474,66 +495,140 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
     for (int d = 0; d < DT; ++d) vr[d] = load16(r, v_at + 1024 * (d & 3), 4096 * (d >> 2));
   };
 
-  for (int p0 = pb + wave; p0 < pe; p0 += 64 * W) {
-    if (!listed || p0 != pb + wave) lp = list(p0 + W * lane, pe, page);
-    if (page >= a.num_pages || lp * static_cast<int64_t>(kPageTokens) > pmax) page = -1;
-    float ks, vs;
-    page_scales(a, h, D, page, ks, vs);
-    uint64_t todo = __ballot(page >= 0);
-    if (!todo) continue;
-    uint4 kr[4][S], vr[DT];
-    int at = __builtin_ctzll(todo);
-    load_k(__builtin_amdgcn_readlane(page, at), kr);
-    load_v(__builtin_amdgcn_readlane(page, at), vr);
-    while (true) {
-      todo &= todo - 1;
-      const int next = todo ? __builtin_ctzll(todo) : -1;
-      const int next_page = __builtin_amdgcn_readlane(page, next < 0 ? at : next);
-      const int first = __builtin_amdgcn_readlane(lp, at) * kPageTokens;
-      const float kscale = lane_value(ks, at), vscale = lane_value(vs, at);
+  int last_token = pmax;  // that the rows which read these pages see
+  auto walk = [&](int pb, int pe) {
+    for (int p0 = pb + wave; p0 < pe; p0 += 64 * W) {
+      if (!listed || p0 != pb + wave) lp = list(p0 + W * lane, pe, page);
+      if (page >= a.num_pages || lp * static_cast<int64_t>(kPageTokens) > last_token) page = -1;
+      float ks, vs;
+      page_scales(a, h, D, page, ks, vs);
+      uint64_t todo = __ballot(page >= 0);
+      if (!todo) continue;
+      uint4 kr[4][S], vr[DT];
+      int at = __builtin_ctzll(todo);
+      load_k(__builtin_amdgcn_readlane(page, at), kr);
+      load_v(__builtin_amdgcn_readlane(page, at), vr);
+      while (true) {
+        todo &= todo - 1;
+        const int next = todo ? __builtin_ctzll(todo) : -1;
+        const int next_page = __builtin_amdgcn_readlane(page, next < 0 ? at : next);
+        const int first = __builtin_amdgcn_readlane(lp, at) * kPageTokens;
+        const float kscale = lane_value(ks, at), vscale = lane_value(vs, at);
 
-      f32x4 x[NT][4] = {};
+        f32x4 x[NT][4] = {};
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
+        for (int s = 0; s < S; ++s) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bf16x8 k0 = fp8x8_to_bf16(kr[j][s].x, kr[j][s].y, 1.0f), k1 = fp8x8_to_bf16(kr[j][s].z, kr[j][s].w, 1.0f);
+          for (int j = 0; j < 4; ++j) {
+            const bf16x8 k0 = fp8x8_to_bf16(kr[j][s].x, kr[j][s].y, 1.0f), k1 = fp8x8_to_bf16(kr[j][s].z, kr[j][s].w, 1.0f);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const bf16x8 q0 = kQLds ? sq[64 * (nt * 2 * S + 2 * s) + lane] : q[kQLds ? 0 : nt][2 * s];
+              const bf16x8 q1 = kQLds ? sq[64 * (nt * 2 * S + 2 * s + 1) + lane] : q[kQLds ? 0 : nt][2 * s + 1];
+              x[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q0, x[nt][j], 0, 0, 0);
+              x[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q1, x[nt][j], 0, 0, 0);
+            }
+            if (j & 1) __builtin_amdgcn_sched_barrier(0);  // few converted pieces at a time
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // the next page goes to the registers that the products above read
+        if (next >= 0) load_k(next_page, kr);
+        __builtin_amdgcn_sched_barrier(0);
+        const bool whole = first + kPageTokens - 1 <= rr.pany && (!a.window || first > pmax - a.window);
+        if (SHARE) {
+          const bool mine = (__builtin_amdgcn_readlane(listing, at) >> n) & 1;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[0][j][i] = mine ? x[0][j][i] : -__builtin_inff();
+          }
+        }
+        bf16x8 w[NT][2];
+        softmax_page<false, NT, DT>(x, kscale, whole, first, g, rr, m, l, o, w);
+        if (!whole) {
+          const uint4 keep = v_keep(first, low, last_token, g);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) vr[d] = and4(vr[d], keep);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const bf16x8 v0 = fp8x8_to_bf16(vr[d].x, vr[d].y, vscale), v1 = fp8x8_to_bf16(vr[d].z, vr[d].w, vscale);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const bf16x8 q0 = kQLds ? sq[64 * (nt * 2 * S + 2 * s) + lane] : q[kQLds ? 0 : nt][2 * s];
-            const bf16x8 q1 = kQLds ? sq[64 * (nt * 2 * S + 2 * s + 1) + lane] : q[kQLds ? 0 : nt][2 * s + 1];
-            x[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q0, x[nt][j], 0, 0, 0);
-            x[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q1, x[nt][j], 0, 0, 0);
+            o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, w[nt][0], o[nt][d], 0, 0, 0);
+            o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, w[nt][1], o[nt][d], 0, 0, 0);
           }
-          if (j & 1) __builtin_amdgcn_sched_barrier(0);  // few converted pieces at a time
+          if (d & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (next < 0) break;
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(next_page, vr);
+        at = next;
+      }
+    }
+  };
+  if constexpr (!SHARE) {
+    walk(pb, pe);
+  } else {
+    // Runs of tokens of one request, ranges of its pages, and, where a list names
+    // a page again, its further mentions: the rows that list each page, and the
+    // pages in order.  Every branch around a barrier is the whole workgroup's.
+    const int toks = rows / a.group, entries = toks * a.n_ids;
+    for (int s0 = 0, s1; s0 < toks; s0 = s1) {
+      b = a.req_ids[t0 + s0];
+      for (s1 = s0 + 1; s1 < toks && a.req_ids[t0 + s1] == b;) ++s1;
+      if (b < 0 || b >= a.num_seqs) continue;
+      bt = a.block_table + b * a.bt_stride;
+      last_token = -1;  // of this run: what lies behind may be anything, and 0 NaN is no 0
+      for (int i = s0; i < s1; ++i) {
+        const int64_t last = min(a.positions[t0 + i], static_cast<int64_t>(0x3fffffff));
+        last_token = max(last_token, static_cast<int>(max(last, static_cast<int64_t>(-1))));
+      }
+      const int np = last_token < 0 ? 0 : min(last_token / kPageTokens + 1, a.bt_width);
+      for (base = 0; base < np; base += kRange) {
+        const int here = min(kRange, np - base), groups = (here + 63) / 64;
+        uint32_t left = 0xffffffffu;  // entries of this thread that are not in yet
+        while (true) {
+          for (int i = tid; i < 64 * groups; i += 64 * W) row_mask[i] = 0;
+          __syncthreads();
+          for (int i = 0, e = tid; e < entries; ++i, e += 64 * W) {
+            const int tok = e / a.n_ids;
+            if (!(left >> i & 1) || tok < s0 || tok >= s1) {
+              left &= ~(1u << i);
+              continue;
+            }
+            const int id = a.ids[(t0 + tok) * a.ids_tok_stride + h * a.ids_head_stride + e - tok * a.n_ids] - base;
+            const uint32_t bits = ((1u << a.group) - 1) << (tok * a.group);
+            if (id < 0 || id >= here || !(atomicOr(&row_mask[id], bits) & bits)) left &= ~(1u << i);
+          }
+          left &= entries > tid ? 0xffffffffu >> (31 - (entries - 1 - tid) / (64 * W)) : 0u;
+          const int again = __syncthreads_or(left != 0);
+          for (int c = wave; c < groups; c += W) {
+            const int some = static_cast<int>(__builtin_popcountll(__ballot(row_mask[64 * c + lane] != 0)));
+            if (lane == 0) counts[c] = some;
+          }
+          __syncthreads();
+          int upto = lane < groups ? counts[lane] : 0;
+#pragma unroll
+          for (int k = 1; k < kRange / 64; k <<= 1) {
+            const int v = __shfl_up(upto, k, 64);
+            if (lane >= k) upto += v;
+          }
+          const int total = __builtin_amdgcn_readlane(upto, kRange / 64 - 1);
+          for (int c = wave; c < groups; c += W) {
+            const bool in = row_mask[64 * c + lane] != 0;
+            const uint64_t all = __ballot(in);
+            const int before = c ? __builtin_amdgcn_readlane(upto, c - 1) : 0;
+            if (in) joined[before + __builtin_popcountll(all & ((1ull << lane) - 1))] = static_cast<uint16_t>(64 * c + lane);
+          }
+          __syncthreads();
+          share = (total + p.parts - 1) / p.parts;
+          walk(p.part * share, min((p.part + 1) * share, total));
+          __syncthreads();
+          if (!again) break;
         }
       }
-      __builtin_amdgcn_sched_barrier(0);  // the next page goes to the registers that the products above read
-      if (next >= 0) load_k(next_page, kr);
-      __builtin_amdgcn_sched_barrier(0);
-      const bool whole = first + kPageTokens - 1 <= rr.pany && (!a.window || first > pmax - a.window);
-      bf16x8 w[NT][2];
-      softmax_page<false, NT, DT>(x, kscale, whole, first, g, rr, m, l, o, w);
-      if (!whole) {
-        const uint4 keep = v_keep(first, low, pmax, g);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vr[d] = and4(vr[d], keep);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const bf16x8 v0 = fp8x8_to_bf16(vr[d].x, vr[d].y, vscale), v1 = fp8x8_to_bf16(vr[d].z, vr[d].w, vscale);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, w[nt][0], o[nt][d], 0, 0, 0);
-          o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, w[nt][1], o[nt][d], 0, 0, 0);
-        }
-        if (d & 1) __builtin_amdgcn_sched_barrier(0);
-      }
-      if (next < 0) break;
-      __builtin_amdgcn_sched_barrier(0);
-      load_v(next_page, vr);
-      at = next;
     }
   }
 
@@ -550,6 +645,7 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
     const int row = (tid >> 4) & 15, r = r0 + 16 * nt + row;
     if (r >= rows) continue;
     const int64_t t = t0 + r / a.group;
+    if (SHARE && (a.req_ids[t] < 0 || a.req_ids[t] >= a.num_seqs)) continue;
     const int hq = h * a.group + r % a.group;
     const float sink = a.sinks ? a.sinks[hq] : 0.0f;
     float top = kNone, sum = 0.0f, f[W];
@@ -818,7 +914,8 @@ struct GqaPlan {
 // head has in each at most, and in all; pages_of(n): the most pages that n
 // consecutive rows see.
 template <typename Pages>
-static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int64_t all_rows, int kv_heads, int dim, bool list, Pages pages_of) {
+static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int64_t all_rows, int kv_heads, int dim, bool list, Pages pages_of,
+                        bool whole_rounds = false) {
   GqaPlan p{};
   const int most = dim == 256 ? 1 : dim == 128 ? 2 : 4;
   // The kernel of few rows streams a page once for 16 row_tiles rows, what the
@@ -875,8 +972,8 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int64_t all_rows, int kv_hea
   // 8), longer ones where each CU has one already (32 of 1,000: 50 us in two
   // parts of 8, 35 in one).
   const int64_t least = p.row_tiles < 8 ? 4 : p.units < 256 ? 8 : 32;
-  int64_t splits = std::min<int64_t>({(round + p.units - 1) / std::max<int64_t>(p.units, 1), (pages + least - 1) / least,
-                                      kMaxSplits});
+  int64_t splits = std::min<int64_t>({(round + (whole_rounds ? 0 : p.units - 1)) / std::max<int64_t>(p.units, 1),
+                                      (pages + least - 1) / least, kMaxSplits});
   splits = std::max<int64_t>(splits, 1);
   p.split_pages = static_cast<int>((pages + splits - 1) / splits);
   p.splits = static_cast<int>((pages + p.split_pages - 1) / p.split_pages);
@@ -917,6 +1014,30 @@ static GqaPlans block_plans(int64_t num_tokens, int group, int kv_heads, int dim
   return p;
 }
 
+// Tokens whose lists a workgroup joins: 16 rows of them, where these are four or
+// more, their sequences have several such tiles and the tiles fill half of the
+// chip.  Lists that agree in nothing but what chance and the forced pages give, 8
+// kv heads of 128, apart and joined, with the selection, in us: 290 rows of 32
+// pages at 6,000 tokens, 1 head a kv head, 134 and 64; 236 at 14,621, 2 heads, 113
+// and 85; 256 at 131,072, 64 pages, 4 heads, 236 and 227.  Below: pairs (8 heads,
+// 200 rows at 48,000) 110 and 123; few tiles (70 rows of 1 kv head) 21 and 28; at
+// 64 channels a page's read is short against the joining (256 rows of 4 kv heads
+// at 20,000, 2 heads) 36 and 44.
+static int shared_tokens(int64_t num_tokens, int64_t num_seqs, int kv_heads, int group, int dim, int64_t num_blocks) {
+  const int share = 16 / group;
+  return share >= 4 && 16 % group == 0 && dim > 64 && num_blocks <= kShareIds &&
+                 num_tokens >= std::max<int64_t>(64, 2 * share * num_seqs) && num_tokens / share * kv_heads >= 128
+             ? share
+             : 1;
+}
+
+static GqaPlans shared_plans(int64_t num_tokens, int share, int kv_heads, int dim, int64_t num_blocks) {
+  GqaPlans p{};
+  p.all = gqa_plan((num_tokens + share - 1) / share, 16, num_tokens, kv_heads, dim, true,
+                   [&](int64_t) { return share * num_blocks; }, true);
+  return p;
+}
+
 static int64_t rows_bytes(int64_t num_tokens, int64_t heads) { return (num_tokens * heads * 8 + 15) / 16 * 16; }
 
 // The parts' sums of a launch.
@@ -929,9 +1050,10 @@ static int64_t plan_bytes(const GqaPlans& p, int64_t num_tokens, int64_t heads, 
   return n ? rows_bytes(num_tokens, heads) + n : 0;
 }
 
-template <int D, bool LIST>
+template <int D, Pages P>
 static int launch_decode(const GqaAttnArgs& a, int row_tiles, bool wide, int64_t blocks, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(blocks));
+  constexpr bool LIST = P != kDense;
   if constexpr (!LIST) {
     if (row_tiles == 8) {
       constexpr int kBytes = 2 * (D / 8 + D / 8) * 64 * 16;
@@ -942,13 +1064,13 @@ static int launch_decode(const GqaAttnArgs& a, int row_tiles, bool wide, int64_t
     }
   }
   constexpr int kWide = 4 * kDecodeWaves<D, 1>;
-  if (row_tiles == 1 && wide) gqa_decode_kernel<D, 1, kWide, LIST><<<grid, 64 * kWide, 0, s>>>(a);
-  else if (row_tiles == 1) gqa_decode_kernel<D, 1, 4, LIST><<<grid, 256, 0, s>>>(a);
-  if constexpr (D <= 128) {
-    if (row_tiles == 2) gqa_decode_kernel<D, 2, 4, LIST><<<grid, 256, 0, s>>>(a);
+  if (row_tiles == 1 && wide) gqa_decode_kernel<D, 1, kWide, P><<<grid, 64 * kWide, 0, s>>>(a);
+  else if (row_tiles == 1) gqa_decode_kernel<D, 1, 4, P><<<grid, 256, 0, s>>>(a);
+  if constexpr (D <= 128 && P != kShared) {
+    if (row_tiles == 2) gqa_decode_kernel<D, 2, 4, P><<<grid, 256, 0, s>>>(a);
   }
   if constexpr (D == 64) {
-    if (row_tiles == 4) gqa_decode_kernel<D, 4, 4, LIST><<<grid, 256, 0, s>>>(a);
+    if (row_tiles == 4) gqa_decode_kernel<D, 4, 4, P><<<grid, 256, 0, s>>>(a);
   }
   int rc = ekv_launch_status();
   if (rc || !a.slots) return rc;
@@ -957,7 +1079,7 @@ static int launch_decode(const GqaAttnArgs& a, int row_tiles, bool wide, int64_t
   return ekv_launch_status();
 }
 
-template <bool LIST>
+template <Pages P>
 static int launch_attn(GqaAttnArgs& a, const GqaPlans& plans, int dim, void* workspace, int64_t workspace_bytes,
                        void* stream) {
   // grids of fewer than 2^32 lanes
@@ -983,9 +1105,11 @@ static int launch_attn(GqaAttnArgs& a, const GqaPlans& plans, int dim, void* wor
       a.ws_ml = reinterpret_cast<float2*>(a.ws_o + p.slots * 16 * p.row_tiles * dim);
       sums += slots_bytes(p, dim);
     }
-    if (dim == 64) return launch_decode<64, LIST>(a, p.row_tiles, p.wide, p.slots, s);
-    if (dim == 128) return launch_decode<128, LIST>(a, p.row_tiles, p.wide, p.slots, s);
-    return launch_decode<256, LIST>(a, p.row_tiles, p.wide, p.slots, s);
+    if constexpr (P != kShared) {
+      if (dim == 64) return launch_decode<64, P>(a, p.row_tiles, p.wide, p.slots, s);
+    }
+    if (dim == 128) return launch_decode<128, P>(a, p.row_tiles, p.wide, p.slots, s);
+    return launch_decode<256, P>(a, p.row_tiles, p.wide, p.slots, s);
   };
   if (plans.both) {
     a.few = kFewRows;
@@ -1057,14 +1181,17 @@ extern "C" int ekv_gqa_attention(const uint16_t* q, int64_t q_tok_stride, int64_
   EKV_CHECK(qsl, "null pointer");
   a.qsl = qsl, a.window = window;
   const int64_t rows = std::min(max_query_len, num_tokens);
-  return launch_attn<false>(a, dense_plans(num_tokens, num_seqs, rows, a.group, kv_heads, dim, max_len, window), dim,
+  return launch_attn<kDense>(a, dense_plans(num_tokens, num_seqs, rows, a.group, kv_heads, dim, max_len, window), dim,
                             workspace, workspace_bytes, stream);
 }
 
 extern "C" int64_t ekv_gqa_block_attention_workspace_size(int32_t num_tokens, int32_t heads, int32_t kv_heads,
                                                           int32_t dim, int32_t num_blocks) {
   if (num_tokens <= 0 || kv_heads <= 0 || heads < kv_heads || !gqa_dim(dim)) return 0;
-  return plan_bytes(block_plans(num_tokens, heads / kv_heads, kv_heads, dim, num_blocks), num_tokens, heads, dim);
+  const int group = heads / kv_heads, share = shared_tokens(num_tokens, 1, kv_heads, group, dim, num_blocks);
+  const int64_t n = plan_bytes(block_plans(num_tokens, group, kv_heads, dim, num_blocks), num_tokens, heads, dim);
+  if (share < 2) return n;
+  return std::max(n, plan_bytes(shared_plans(num_tokens, share, kv_heads, dim, num_blocks), num_tokens, heads, dim));
 }
 
 extern "C" int ekv_gqa_block_attention(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride,
@@ -1086,6 +1213,12 @@ extern "C" int ekv_gqa_block_attention(const uint16_t* q, int64_t q_tok_stride, 
   EKV_CHECK(req_ids && (blocks || !num_blocks), "null pointer");
   a.req_ids = req_ids, a.ids = blocks, a.ids_tok_stride = blocks_tok_stride, a.ids_head_stride = blocks_head_stride;
   a.n_ids = num_blocks;
-  return launch_attn<true>(a, block_plans(num_tokens, a.group, kv_heads, dim, num_blocks), dim, workspace, workspace_bytes,
-                           stream);
+  const int share = shared_tokens(num_tokens, num_seqs, kv_heads, a.group, dim, num_blocks);
+  if (share > 1) {
+    a.share = share;
+    return launch_attn<kShared>(a, shared_plans(num_tokens, share, kv_heads, dim, num_blocks), dim, workspace,
+                                workspace_bytes, stream);
+  }
+  return launch_attn<kList>(a, block_plans(num_tokens, a.group, kv_heads, dim, num_blocks), dim, workspace,
+                            workspace_bytes, stream);
 }
