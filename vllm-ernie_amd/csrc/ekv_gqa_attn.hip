@@ -362,7 +362,8 @@ __device__ __forceinline__ void page_scales(const GqaAttnArgs& a, int h, int dim
 // q leaves a lane the scores of one row and of the tokens whose V bytes it
 // loads, so the weights go straight into the product with V.  The next page's K
 // and V are asked for as soon as the products that read their registers are
-// issued.
+// issued.  Lists of neighbouring rows may be joined: each page that any of them
+// names is read once, and a mask says which rows it counts for.
 //
 // Bound by the read of the pages (32 rows of 64 heads at 131,072 tokens, 8 kv
 // heads of 128: 8.6 GB in 1,412 us, 6.1 TB/s; 13 sequences of 2,000 to 48,000:
