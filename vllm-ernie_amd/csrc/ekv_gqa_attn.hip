@@ -971,8 +971,10 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int64_t all_rows, int kv_hea
   // Pages of a part.  Of many rows: shorter parts where units are fewer than CUs
   // (4 sequences of 4,096 tokens, 16 rows, 8 kv heads of 128: 37 us at 16, 31 at
   // 8), longer ones where each CU has one already (32 of 1,000: 50 us in two
-  // parts of 8, 35 in one).
-  const int64_t least = p.row_tiles < 8 ? 4 : p.units < 256 ? 8 : 32;
+  // parts of 8, 35 in one), the shortest where most CUs have none (5 of 931 tokens,
+  // 8 rows of 12 heads a kv head of 256: 31 us at 8, 22 at 4; 224 units of 12
+  // pages: 47 and 51; the 4 of 4,096 again: 31 and 33).
+  const int64_t least = p.row_tiles < 8 || (p.units < 64 && pages >= 12 && pages <= 48) ? 4 : p.units < 256 ? 8 : 32;
   int64_t splits = std::min<int64_t>({(round + (whole_rounds ? 0 : p.units - 1)) / std::max<int64_t>(p.units, 1),
                                       (pages + least - 1) / least, kMaxSplits});
   splits = std::max<int64_t>(splits, 1);
