@@ -27,7 +27,6 @@ its work is the same for every seed.
 
 from __future__ import annotations
 
-import functools
 import math
 import random
 import sys
@@ -43,10 +42,10 @@ KEEP_FIRST, KEEP_LAST = 1, 2  # blocks that every row attends to: the first, and
 F64 = torch.float64
 
 
-@functools.lru_cache(maxsize=None)
 def _ops():
-    """The framework's wrappers, imported at the first call: a program imports them once."""
-    sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "vllm-ernie_amd"))
+    root = str(Path(__file__).resolve().parents[1] / "vllm-ernie_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
     from ernie_kv import ops
 
     return ops
