@@ -15,10 +15,19 @@ namespace ekv {
 constexpr float kLog2e = 0x1.715476p+0f;
 constexpr float kLn2 = 0x1.62e430p-1f;
 constexpr float kNone = -1e30f;   // reference of a row that has seen no token
-constexpr float kMoveAt = 4096.0f; // weight, or sum of a lane's 16, that moves a row's reference
+// Weights are rounded to fp16 (11 bits, up to 65,504) for the product with V;
+// as bf16 their rounding was the largest error of a result (1.4 times that of
+// 32-bit weights, for 2% less time at 4,096 rows).  A reference lies 2^kLift
+// below the largest score: weights of 2^-19 of the largest keep all bits, those
+// down to 2^-30 some, and up to kMoveAt the reference stays (2^9 below it, and so
+// moved sooner: 1% more time at 4,096 rows).
+constexpr int kLift = 5;
+constexpr float kMoveAt = 32768.0f; // weight, or sum of a lane's 16, that moves a row's reference
 constexpr int kMaxSplits = 64;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct GqaAttnArgs {
   const uint16_t* q;
@@ -153,6 +162,61 @@ __device__ __forceinline__ bf16x8 fp8x8_to_bf16(uint32_t lo, uint32_t hi, float 
                                                __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)));
 }
 
+// The same as fp16: exact while the power of two is 2^-15 to 2^7.
+__device__ __forceinline__ f16x8 fp8x8_to_f16(uint32_t lo, uint32_t hi, float s) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s, true);
+  return __builtin_bit_cast(f16x8, make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                                              __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)));
+}
+
+// The sums o are held in units of 2^at, in which a page's values are codes times
+// 2^-15 to 2^7: most pages' scales are within that of the first one's.  A page
+// whose scale is not moves the unit, and the sums with it; `top` is the largest
+// scale so far, 2^64 below which no unit goes, as the sums would overflow (values
+// 2^-75 of the largest ones' are taken as zeros there).
+struct ValueUnit {
+  int at = -1000, top = -1000;
+};
+
+// The power of two that V's codes of a page with scale vscale (wave-uniform) are
+// taken by; a page of scale 0 holds zeros.
+template <int NT, int DT>
+__device__ __forceinline__ float value_factor(float vscale, ValueUnit& unit, f32x4 (&o)[NT][DT]) {
+  const int e = (__builtin_bit_cast(int, vscale) >> 23) - 127;
+  if (e == -127) return 0x1p-100f;
+  if (e - unit.at < -15 || e - unit.at > 7) {
+    unit.top = max(unit.top, e);
+    const int to = max(e, unit.top - 64) + 4;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][d][i] = __builtin_ldexpf(o[nt][d][i], unit.at - to);
+      }
+    }
+    unit.at = to;
+  }
+  return exp2i(max(e - unit.at, -100));
+}
+
+// Sums and weights' sums as they are without units and lift.
+template <int NT, int DT>
+__device__ __forceinline__ void plain_units(const ValueUnit& unit, float (&l)[NT], f32x4 (&o)[NT][DT]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    l[nt] *= exp2i(-kLift);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[nt][d][i] = __builtin_ldexpf(o[nt][d][i], unit.at - kLift);
+    }
+  }
+}
+
 // 16 bytes at a page's scalar base + the lane's offset + a constant: buffer
 // loads, so that a page's addresses take one register of a lane.
 typedef __amdgpu_buffer_rsrc_t PageRsrc;
@@ -167,11 +231,11 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-// Result of a row whose weights sum to l around the reference m: 4 channels.
+// Result of a row whose weights sum to l around 2^kLift times the reference m: 4 channels.
 __device__ __forceinline__ void store_out4(const GqaAttnArgs& a, int64_t t, int hq, int c, f32x4 o, float m, float l,
                                            float sink) {
   float den = l;
-  if (a.sinks) den += __builtin_amdgcn_exp2f(sink * kLog2e - m);
+  if (a.sinks) den += __builtin_amdgcn_exp2f(sink * kLog2e - m - kLift);
   const float inv = den > 0.0f ? 1.0f / den : (den == den ? 0.0f : den);
   const uint32_t lo = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(o[0] * inv), static_cast<__bf16>(o[1] * inv)});
   const uint32_t hi = __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(o[2] * inv), static_cast<__bf16>(o[3] * inv)});
@@ -180,7 +244,7 @@ __device__ __forceinline__ void store_out4(const GqaAttnArgs& a, int64_t t, int 
 }
 
 __device__ __forceinline__ void store_lse(const GqaAttnArgs& a, int64_t t, int hq, float m, float l) {
-  if (a.lse) a.lse[t * a.lse_stride + hq] = l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (a.lse) a.lse[t * a.lse_stride + hq] = l == 0.0f ? -__builtin_inff() : (m + (__builtin_amdgcn_logf(l) + kLift)) * kLn2;
 }
 
 // Rows of a wave's NT tiles of 16 queries: what each lane's row sees.
@@ -193,14 +257,14 @@ struct RowRange {
 // Scores x (token 16 j + 4 g + i of the page, row n) -> weights around the
 // rows' references m, as the B operand of the product with V, and their sums.
 // kscale > 0 takes a raw score to log2 units.  A reference is a maximum that the
-// row has had, and moves only where the page's weights around it grow past
+// row has had, less kLift, and moves only where the page's weights around it grow past
 // kMoveAt.  kBySum sees that in their sums, which costs no maximum but the raw
 // scores' registers (many rows, where the products bound the kernel: 3% less time
 // at 4,096 rows); else in the largest score.  Masks are selects without branches.
 template <bool kBySum, int NT, int DT>
 __device__ __forceinline__ void softmax_page(f32x4 (&x)[NT][4], float kscale, bool whole, int first, int g,
                                              const RowRange<NT>& r, float (&m)[NT], float (&l)[NT],
-                                             f32x4 (&o)[NT][DT], bf16x8 (&w)[NT][2]) {
+                                             f32x4 (&o)[NT][DT], f16x8 (&w)[NT][2]) {
   if (!whole) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -243,7 +307,7 @@ __device__ __forceinline__ void softmax_page(f32x4 (&x)[NT][4], float kscale, bo
   if (__any(most > kMoveAt)) {  // infinite too: a row's first page, whose reference is none
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float t = fmaxf(kBySum ? largest(nt) : top[nt], m[nt]);
+      float t = fmaxf((kBySum ? largest(nt) : top[nt]) - kLift, m[nt]);
       t = fmaxf(t, __shfl_xor(t, 16, 64));
       t = fmaxf(t, __shfl_xor(t, 32, 64));
       const float f = __builtin_amdgcn_exp2f(m[nt] - t);
@@ -259,7 +323,7 @@ __device__ __forceinline__ void softmax_page(f32x4 (&x)[NT][4], float kscale, bo
     if (!kBySum) weights(nt);
     l[nt] += s[nt];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[nt][i >> 3][i & 7] = static_cast<__bf16>(y[nt][i]);
+    for (int i = 0; i < 16; ++i) w[nt][i >> 3][i & 7] = static_cast<_Float16>(y[nt][i]);
   }
 }
 
@@ -478,6 +542,7 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
   float m[NT], l[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) m[nt] = kNone, l[nt] = 0.0f;
+  ValueUnit units;
 
   const uint8_t* const k_base = a.cache + static_cast<int64_t>(h) * kPageTokens * D;
   const uint32_t v_step = static_cast<uint32_t>(a.kv_heads) * kPageTokens * D;
@@ -544,8 +609,9 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
             for (int i = 0; i < 4; ++i) x[0][j][i] = mine ? x[0][j][i] : -__builtin_inff();
           }
         }
-        bf16x8 w[NT][2];
+        f16x8 w[NT][2];
         softmax_page<false, NT, DT>(x, kscale, whole, first, g, rr, m, l, o, w);
+        const float vfactor = value_factor<NT, DT>(vscale, units, o);
         if (!whole) {
           const uint4 keep = v_keep(first, low, last_token, g);
 #pragma unroll
@@ -554,11 +620,11 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const bf16x8 v0 = fp8x8_to_bf16(vr[d].x, vr[d].y, vscale), v1 = fp8x8_to_bf16(vr[d].z, vr[d].w, vscale);
+          const f16x8 v0 = fp8x8_to_f16(vr[d].x, vr[d].y, vfactor), v1 = fp8x8_to_f16(vr[d].z, vr[d].w, vfactor);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, w[nt][0], o[nt][d], 0, 0, 0);
-            o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, w[nt][1], o[nt][d], 0, 0, 0);
+            o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w[nt][0], o[nt][d], 0, 0, 0);
+            o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w[nt][1], o[nt][d], 0, 0, 0);
           }
           if (d & 1) __builtin_amdgcn_sched_barrier(0);
         }
@@ -634,6 +700,7 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
   }
 
   // the waves' parts of each row
+  plain_units<NT, DT>(units, l, o);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     l[nt] += __shfl_xor(l[nt], 16, 64);
@@ -740,6 +807,7 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
   float m[NT], l[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) m[nt] = kNone, l[nt] = 0.0f;
+  ValueUnit units;
 
   // this wave's part of a page: pieces KT wave .. of K (S of each 16 tokens),
   // channels D / W wave .. of V
@@ -768,7 +836,7 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
     auto stage = [&](int at, int half) {
       bf16x8* const dst = buf + half * kHalf + lane;
       const int first = (p0 + at) * kPageTokens;
-      const float vscale = lane_value(vs, at);
+      const float vfactor = value_factor<NT, DT>(lane_value(vs, at), units, o);
 #pragma unroll
       for (int s = 0; s < KT; ++s) {
         dst[((wave * KT + s) * 2) * 64] = fp8x8_to_bf16(kr[s].x, kr[s].y, 1.0f);
@@ -781,8 +849,8 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
       }
 #pragma unroll
       for (int i = 0; i < VT; ++i) {
-        dst[(8 * S + (wave * VT + i) * 2) * 64] = fp8x8_to_bf16(vr[i].x, vr[i].y, vscale);
-        dst[(8 * S + (wave * VT + i) * 2 + 1) * 64] = fp8x8_to_bf16(vr[i].z, vr[i].w, vscale);
+        dst[(8 * S + (wave * VT + i) * 2) * 64] = __builtin_bit_cast(bf16x8, fp8x8_to_f16(vr[i].x, vr[i].y, vfactor));
+        dst[(8 * S + (wave * VT + i) * 2 + 1) * 64] = __builtin_bit_cast(bf16x8, fp8x8_to_f16(vr[i].z, vr[i].w, vfactor));
       }
     };
     int at = __builtin_ctzll(todo), half = 0;
@@ -811,17 +879,17 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
         }
         __builtin_amdgcn_s_setprio(0);
         const bool whole = first + kPageTokens - 1 <= rr.pany && (!a.window || first > rr.pmax - a.window);
-        bf16x8 w[NT][2];
+        f16x8 w[NT][2];
         softmax_page<true, NT, DT>(x, lane_value(ks, at), whole, first, g, rr, m, l, o, w);
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            const bf16x8 v = src[(8 * S + 2 * d + u) * 64];
+            const f16x8 v = __builtin_bit_cast(f16x8, src[(8 * S + 2 * d + u) * 64]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[nt][u], o[nt][d], 0, 0, 0);
+              o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[nt][u], o[nt][d], 0, 0, 0);
           }
         }
       }
@@ -831,6 +899,7 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
     }
   }
 
+  plain_units<NT, DT>(units, l, o);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     l[nt] += __shfl_xor(l[nt], 16, 64);
