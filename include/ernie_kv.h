@@ -782,7 +782,8 @@ int64_t ekv_gqa_attention_workspace_size(int32_t num_tokens, int32_t num_seqs, i
  *   s_j = scale q . k_j; lse [T, heads] fp32 = log sum_j e^{s_j} (may be NULL).
  * scale > 0, finite; sinks [heads] fp32 may be NULL.  A row that sees no token (a negative
  * position) gets zeros and -inf; rows of no sequence are left as they were.
- * max_query_len and max_len bound the rows and the tokens of a sequence.  What
+ * max_query_len and max_len bound the rows and the tokens of a sequence (heads of
+ * rows past max_query_len are computed like the others or left as they were).  What
  * lies behind a sequence's last token is never used, whatever its bytes.
  * workspace (16-byte aligned) holds the partial results of long sequences;
  * calls that share one must not overlap.

@@ -1,0 +1,77 @@
+"""GPU: calls of grouped-query attention that several kernels or parts share:
+bounds below a call's rows, workspaces that another call has used, single rows
+and drafts beside chunks -- against the oracle."""
+
+import numpy as np
+import pytest
+import torch
+
+from helpers import bf16_tensor, bf16_values, randn_bf16, to_dev
+from oracle import gqa
+from test_gpu_gqa import Layer, check_rows
+
+pytestmark = pytest.mark.gpu
+
+
+def batch(rng, lens, rows, H, D):
+    q = randn_bf16(rng, (sum(rows), H, D))
+    pos = np.concatenate([np.arange(n - r, n) for n, r in zip(lens, rows)]).astype(np.int64)
+    return q, pos, np.repeat(np.arange(len(lens)), rows), np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+
+
+def call(layer, q, pos, qsl, most, max_len, window=0, sinks=None, workspace=None, bt=None):
+    from ernie_kv import ops
+
+    dev, (T, H, D) = layer.dev, q.shape
+    out = torch.full((T, H, D), 7.0, dtype=torch.bfloat16, device=dev)
+    lse = torch.full((T, H), 7.0, device=dev)
+    ops.gqa_attention(bf16_tensor(q, dev), layer.d_cache, layer.KV, layer.d_bt if bt is None else bt, to_dev(pos, dev),
+                      to_dev(qsl, dev), most, max_len, D ** -0.5, out, lse, sinks=None if sinks is None else to_dev(sinks, dev),
+                      window=window, workspace=workspace)
+    return bf16_values(out).astype(np.float64), lse.cpu().numpy()
+
+
+def size(q, qsl, most, max_len, KV, window=0):
+    """Workspace bytes that a call of these bounds needs."""
+    from ernie_kv import _lib
+
+    return _lib.load().ekv_gqa_attention_workspace_size(q.shape[0], len(qsl) - 1, most, max_len, q.shape[1], KV, q.shape[2],
+                                                        window)
+
+
+@pytest.mark.parametrize("D,H,KV", [(64, 12, 2), (128, 8, 1), (256, 16, 2)])
+@pytest.mark.parametrize("lens,rows,told", [([2000], [9], 1), ([2000], [2], 1), ([2000, 700, 1000], [7, 11, 0], 1),
+                                            ([2000, 900], [90, 200], 30), ([2000], [400], 120),
+                                            ([2000, 300, 1000, 66], [40, 1, 300, 2], 20)])
+def test_rows_past_the_bound(dev, D, H, KV, lens, rows, told):
+    """More rows in a sequence than max_query_len says, in a workspace that holds
+    other calls' records: rows within the bound are right, each head of those past
+    it is right too or left as it was."""
+    rng = np.random.default_rng(D + told + sum(rows))
+    layer = Layer(dev, rng, lens, KV, D, summary=False)
+    q, pos, seq, qsl = batch(rng, lens, rows, H, D)
+    need, most = size(q, qsl, told, 9000, KV), max(rows)  # a bound of lengths far above them: parts of few pages
+    assert need
+    seen = lambda t, h: np.arange(pos[t] + 1)  # noqa: E731
+    sure = [t for t in range(len(pos)) if t - qsl[seq[t]] < told]
+    some = sorted(set(sure[:6] + sure[-6:]) | set(int(t) for t in rng.integers(0, len(pos), 12)) | {len(pos) - 1})
+    held, refs = [gqa.tokens(layer.cache, layer.bt[b][:-1], KV, D, h) for b in range(len(lens)) for h in range(KV)], {}
+
+    def ref(t, hq):
+        if (t, hq) not in refs:
+            keys, vals = held[seq[t] * KV + hq * KV // H]
+            refs[t, hq] = gqa.attend(q[t, hq], keys[:pos[t] + 1], vals[:pos[t] + 1], D ** -0.5)[:2]
+        return refs[t, hq]
+
+    for left in (2, 1 << 8 | 3, 1 << 16 | 2, "a call"):
+        n = max(need, size(q, qsl, most, 9000, KV)) // 4 + 1
+        ws = torch.full((n,), 0 if left == "a call" else left, dtype=torch.int32, device=dev).view(torch.uint8)
+        if left == "a call":
+            call(layer, q, pos, qsl, most, 9000, workspace=ws)
+        out, lse = call(layer, q, pos, qsl, told, 9000, workspace=ws)
+        kept = (out == 7).all(2) & (lse == 7)
+        assert not kept[sure].any()
+        for t, hq in zip(*np.nonzero(kept)):
+            if t in some:
+                out[t, hq], lse[t, hq] = ref(t, hq)
+        check_rows(layer, q, out, lse, D ** -0.5, [(t, seq[t]) for t in some], None, seen)

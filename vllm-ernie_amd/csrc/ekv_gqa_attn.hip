@@ -7,6 +7,7 @@
 // over the tokens j a row sees: j <= position and, with a window,
 // j > position - window.
 #include <algorithm>
+#include <type_traits>
 
 #include "ekv_gqa.h"
 
@@ -419,6 +420,14 @@ __device__ __forceinline__ void page_scales(const GqaAttnArgs& a, int h, int dim
   }
 }
 
+// Rows `from` .. rows - 1 of a sequence, which no workgroup takes (it has more than
+// the call said), name no part: what a workspace holds of an earlier call is not
+// this one's.
+__device__ __forceinline__ void name_no_parts(const GqaAttnArgs& a, int t0, int h, int from, int rows, int step) {
+  for (int r = from + static_cast<int>(threadIdx.x); r < rows; r += step)
+    a.ws_rows[(t0 + r / a.group) * static_cast<int64_t>(a.heads) + h * a.group + r % a.group] = make_int2(0, a.kind << 16);
+}
+
 // ---------------------------------------------------------------------------
 // Few rows a kv head: one workgroup per (16 NT rows, kv head, range of pages).
 // Each of its W waves takes every W-th page of the range through registers,
@@ -739,6 +748,7 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
         a.ws_rows[t * a.heads + hq] = make_int2(p.first, p.parts | (16 * nt + row) << 8 | a.kind << 16);
     }
   }
+  if (P == kDense && a.ws_rows && p.part == 0 && p.tile == a.tiles - 1) name_no_parts(a, t0, h, r0 + 16 * NT, rows, 64 * W);
 }
 
 // ---------------------------------------------------------------------------
@@ -922,6 +932,7 @@ __global__ void __launch_bounds__(64 * PrefillShape<D>::kWaves, 2) gqa_prefill_k
         a.ws_rows[t * a.heads + hq] = make_int2(unit, a.splits | (16 * (NT * wave + nt) + n) << 8 | a.kind << 16);
     }
   }
+  if (a.ws_rows && split == 0 && !a.by_rows && tile == a.tiles - 1) name_no_parts(a, t0, h, (tile + 1) * 128, rows, 64 * W);
 }
 
 // Joins a row's parts: out = sum_p e^(m_p - m) o_p / sum_p e^(m_p - m) l_p, one
@@ -939,9 +950,9 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a, int slo
   const int lo = LIST ? a.req_ids[t] : a.qsl[0], hi = LIST ? a.num_seqs : a.qsl[a.num_seqs];
   if (LIST ? lo < 0 || lo >= hi : t < lo || t >= hi) return;
   const int parts = info.y & 255, at = (info.y >> 8) & 255;
-  // whole already, or the other kernel's; and a row that no workgroup took (more of them than the call said) names no part
-  if (parts < 2 || info.y >> 16 != a.kind || parts > kMaxSplits || at >= slot_rows || info.x < 0 ||
-      info.x + static_cast<int64_t>(parts - 1) * a.part_step >= a.slots)
+  if (parts < 2 || info.y >> 16 != a.kind) return;  // whole already, no workgroup's, or the other kernel's
+  // offsets that do not ascend may leave a row out; whatever the workspace holds, no read leaves it
+  if (parts > kMaxSplits || at >= slot_rows || info.x < 0 || info.x + static_cast<int64_t>(parts - 1) * a.part_step >= a.slots)
     return;
   const int64_t first = static_cast<int64_t>(info.x) * slot_rows + at, step = static_cast<int64_t>(a.part_step) * slot_rows;
   float2 ml = make_float2(kNone, 0.0f);
@@ -1122,8 +1133,9 @@ static int64_t plan_bytes(const GqaPlans& p, int64_t num_tokens, int64_t heads, 
   return n ? rows_bytes(num_tokens, heads) + n : 0;
 }
 
+// The kernel of a plan.
 template <int D, Pages P>
-static int launch_decode(const GqaAttnArgs& a, int row_tiles, bool wide, int64_t blocks, hipStream_t s) {
+static int launch_parts(const GqaAttnArgs& a, int row_tiles, bool wide, int64_t blocks, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(blocks));
   constexpr bool LIST = P != kDense;
   if constexpr (!LIST) {
@@ -1144,10 +1156,14 @@ static int launch_decode(const GqaAttnArgs& a, int row_tiles, bool wide, int64_t
   if constexpr (D == 64) {
     if (row_tiles == 4) gqa_decode_kernel<D, 4, 4, P><<<grid, 256, 0, s>>>(a);
   }
-  int rc = ekv_launch_status();
-  if (rc || !a.slots) return rc;
+  return ekv_launch_status();
+}
+
+// The join of its parts.
+template <int D, Pages P>
+static int launch_join(const GqaAttnArgs& a, int row_tiles, hipStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.heads;
-  gqa_combine_kernel<D, LIST><<<dim3(static_cast<uint32_t>((rows + 3) / 4)), 256, 0, s>>>(a, 16 * row_tiles);
+  gqa_combine_kernel<D, P != kDense><<<dim3(static_cast<uint32_t>((rows + 3) / 4)), 256, 0, s>>>(a, 16 * row_tiles);
   return ekv_launch_status();
 }
 
@@ -1155,9 +1171,9 @@ template <Pages P>
 static int launch_attn(GqaAttnArgs& a, const GqaPlans& plans, int dim, void* workspace, int64_t workspace_bytes,
                        void* stream) {
   // grids of fewer than 2^32 lanes
-  const bool join = plans.all.join || plans.few.join;
+  const bool joins = plans.all.join || plans.few.join;
   EKV_CHECK(plans.all.slots < (1 << 23) && plans.few.slots < (1 << 23) &&
-                (!join || static_cast<int64_t>(a.num_tokens) * a.heads < (1 << 26)),
+                (!joins || static_cast<int64_t>(a.num_tokens) * a.heads < (1 << 26)),
             "too many rows for one call");
   const int64_t need = plan_bytes(plans, a.num_tokens, a.heads, dim);
   if (need > workspace_bytes || (need && !workspace)) {
@@ -1168,28 +1184,39 @@ static int launch_attn(GqaAttnArgs& a, const GqaPlans& plans, int dim, void* wor
   if (need) a.ws_rows = static_cast<int2*>(workspace);
   uint8_t* sums = static_cast<uint8_t*>(workspace) + rows_bytes(a.num_tokens, a.heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  auto launch = [&](const GqaPlan& p) {
+  auto by_dim = [&](auto run) {
+    if constexpr (P != kShared) {
+      if (dim == 64) return run(std::integral_constant<int, 64>{});
+    }
+    if (dim == 128) return run(std::integral_constant<int, 128>{});
+    return run(std::integral_constant<int, 256>{});
+  };
+  auto parts = [&](const GqaPlan& p) {
     a.tiles = p.tiles, a.units = static_cast<int32_t>(p.units), a.splits = p.splits, a.split_pages = p.split_pages;
-    a.budget = p.budget, a.by_rows = p.by_rows, a.slots = 0;
+    a.budget = p.budget, a.by_rows = p.by_rows;
     if (p.join) {
       a.slots = static_cast<int32_t>(p.slots), a.part_step = p.budget ? a.kv_heads * p.tiles : a.units;
       a.ws_o = reinterpret_cast<float*>(sums);
       a.ws_ml = reinterpret_cast<float2*>(a.ws_o + p.slots * 16 * p.row_tiles * dim);
       sums += slots_bytes(p, dim);
     }
-    if constexpr (P != kShared) {
-      if (dim == 64) return launch_decode<64, P>(a, p.row_tiles, p.wide, p.slots, s);
-    }
-    if (dim == 128) return launch_decode<128, P>(a, p.row_tiles, p.wide, p.slots, s);
-    return launch_decode<256, P>(a, p.row_tiles, p.wide, p.slots, s);
+    return by_dim([&](auto d) { return launch_parts<d(), P>(a, p.row_tiles, p.wide, p.slots, s); });
   };
-  if (plans.both) {
-    a.few = kFewRows;
-    const int rc = launch(plans.few);
-    if (rc) return rc;
-    a.kind = 1;
+  auto join = [&](const GqaAttnArgs& of, const GqaPlan& p) {
+    return p.join ? by_dim([&](auto d) { return launch_join<d(), P>(of, p.row_tiles, s); }) : kOk;
+  };
+  if (!plans.both) {
+    const int rc = parts(plans.all);
+    return rc ? rc : join(a, plans.all);
   }
-  return launch(plans.all);
+  // joins last: by then each row says which kernel it is of
+  a.few = kFewRows;
+  int rc = parts(plans.few);
+  const GqaAttnArgs few = a;
+  a.kind = 1;
+  if (!rc) rc = parts(plans.all);
+  if (!rc) rc = join(few, plans.few);
+  return rc ? rc : join(a, plans.all);
 }
 
 static int attn_args(GqaAttnArgs& a, const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride,
