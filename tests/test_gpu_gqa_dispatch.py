@@ -75,3 +75,56 @@ def test_rows_past_the_bound(dev, D, H, KV, lens, rows, told):
             if t in some:
                 out[t, hq], lse[t, hq] = ref(t, hq)
         check_rows(layer, q, out, lse, D ** -0.5, [(t, seq[t]) for t in some], None, seen)
+
+
+def shared_call(dev, D, H, KV, lens, rows, window=0, held=None, max_len=1 << 20):
+    """A call that both kernels may share, checked against the oracle; (parts,
+    kernel) of each row, 0 the kernel of few rows, as the workspace names them.
+    held: the sequences with pages of their own, of which the others read some."""
+    rng = np.random.default_rng(D + H + sum(rows))
+    held = list(range(len(lens))) if held is None else held
+    layer = Layer(dev, rng, [lens[b] for b in held], KV, D, summary=False)
+    bt = np.full((len(lens), layer.bt.shape[1]), -1, np.int32)
+    bt[:] = layer.bt[rng.integers(0, len(held), len(lens))]
+    bt[held] = layer.bt
+    q, pos, seq, qsl = batch(rng, lens, rows, H, D)
+    sinks = rng.standard_normal(H).astype(np.float32)
+    n = size(q, qsl, max(rows), max_len, KV, window)
+    assert n, "one kernel, no parts"
+    some = [t for t in range(len(pos)) if seq[t] in held and rows[seq[t]] < 20]
+    some += [int(t) for b in held if rows[b] >= 20 for t in (qsl[b], qsl[b + 1] - 1, *rng.integers(qsl[b], qsl[b + 1], 5))]
+    for left in (2, -1):
+        ws = torch.full((n // 4 + 1,), left, dtype=torch.int32, device=dev).view(torch.uint8)
+        out, lse = call(layer, q, pos, qsl, max(rows), max_len, window, sinks, ws, to_dev(bt, dev))
+        check_rows(layer, q, out, lse, D ** -0.5, [(t, held.index(seq[t])) for t in some], sinks,
+                   lambda t, h: np.arange(max(0, pos[t] - window + 1) if window else 0, pos[t] + 1))
+    y = ws[:8 * len(pos) * H].view(torch.int32).view(len(pos), H, 2)[..., 1].cpu().numpy()
+    return y & 255, y >> 16, np.array(rows)[seq]
+
+
+@pytest.mark.parametrize("D,H,KV", [(64, 8, 1), (128, 8, 1), (128, 12, 4), (256, 8, 1)])
+@pytest.mark.parametrize("lens,rows", [([9000, 600], [1, 500]), ([700, 9000, 5000], [500, 1, 500]),
+                                       ([3000, 400, 900, 20, 2000], [1, 400, 300, 1, 1])])
+@pytest.mark.parametrize("window", [0, 100_000])
+def test_a_single_row_beside_a_chunk(dev, D, H, KV, lens, rows, window):
+    """However few they are: single rows go to the kernel of few rows, in parts, where they may see many pages."""
+    parts, kernel, n = shared_call(dev, D, H, KV, lens, rows, window)
+    assert np.all(kernel[n == 1] == 0) and np.all(kernel[n > 1] == 1)
+    assert np.all(parts[(n == 1) & (np.repeat(lens, rows) >= 1000)] > 1)
+
+
+def test_chunks_alone_are_one_launch(dev):
+    """No sequence of a call can be short: no second kernel."""
+    parts, kernel, n = shared_call(dev, 128, 8, 1, [900, 700], [400, 399])
+    assert np.all(kernel == 0)
+
+
+@pytest.mark.parametrize("seqs", [100, 260])
+def test_many_single_rows_beside_a_chunk(dev, seqs):
+    """More than 64 sequences, and more than are shared out by their lengths."""
+    rng = np.random.default_rng(seqs)
+    lens, rows = [int(n) for n in rng.integers(1, 900, seqs)], [1] * seqs
+    lens[7], rows[7], lens[50], rows[60] = 9000, 1, 800, 0
+    rows[50] = 600
+    parts, kernel, n = shared_call(dev, 128, 8, 1, lens, rows, held=sorted({0, 7, 20, 50, 77, seqs - 1}))
+    assert np.all(kernel[n == 1] == 0) and np.all(kernel[n > 1] == 1)

@@ -1066,15 +1066,19 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int64_t all_rows, int kv_hea
 }
 
 // A call's launches: `all`, or where chunks may stand beside single rows that see
-// many pages, the kernel of few rows, in parts, for sequences of up to kFewRows
-// and `all` for the others.  64 heads, 8 kv heads of 128, `all` against both, in
-// us: 8 rows at 131,072 tokens and a chunk of 512 1,433 and 441, 32 at 8,192 and
-// 2,048 371 and 331; at shorter contexts the second launch costs more than it
-// gives: 64 at 2,000 and 4,096 560 and 610, 8 at 1,000 and 1,024 101 and 121.
+// many pages, the kernel of few rows, in parts, for sequences of up to few_rows
+// and `all` for the others.  Not where the kernel of many rows has parts of fewer
+// than 128 pages by itself, whose walk costs about what a second launch does.
+// 64 heads, 8 kv heads of 128, `all` against both, in us: 1 row at 131,072 tokens
+// and a chunk of 512 2,885 and 191, 3 and four chunks of 512 3,060 and 455; 1 at
+// 8,192 and 512 at 1,000 188 and 56; 1 at 8,192 and 512 there too 261 and 264; 1
+// at 8,192 and 64 (parts of 16 pages) 55 and 71, 1 at 32,768 and 64 145 and 172.
 struct GqaPlans {
   GqaPlan all, few;
+  int few_rows;
   bool both;
 };
+
 constexpr int kFewRows = 16;
 
 static GqaPlans dense_plans(int64_t tokens, int64_t seqs, int64_t max_rows, int group, int kv_heads, int dim,
@@ -1086,8 +1090,11 @@ static GqaPlans dense_plans(int64_t tokens, int64_t seqs, int64_t max_rows, int 
   };
   GqaPlans p{};
   p.all = gqa_plan(seqs, max_rows * group, tokens * group, kv_heads, dim, false, pages);
-  p.both = p.all.by_rows && group <= kFewRows && pages(kFewRows) >= 128;
-  if (p.both) p.few = gqa_plan(seqs, kFewRows, tokens * group, kv_heads, dim, false, pages);
+  p.few_rows = group <= kFewRows ? kFewRows : 0;
+  // some sequence may have as few rows, of those that the call has in all
+  const bool some = p.few_rows && tokens <= (seqs - 1) * max_rows + p.few_rows / group;
+  p.both = p.all.row_tiles == 8 && some && pages(p.few_rows) >= 128 * p.all.splits;
+  if (p.both) p.few = gqa_plan(seqs, p.few_rows, tokens * group, kv_heads, dim, false, pages);
   return p;
 }
 
@@ -1210,7 +1217,7 @@ static int launch_attn(GqaAttnArgs& a, const GqaPlans& plans, int dim, void* wor
     return rc ? rc : join(a, plans.all);
   }
   // joins last: by then each row says which kernel it is of
-  a.few = kFewRows;
+  a.few = plans.few_rows;
   int rc = parts(plans.few);
   const GqaAttnArgs few = a;
   a.kind = 1;
