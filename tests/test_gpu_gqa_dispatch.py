@@ -128,3 +128,23 @@ def test_many_single_rows_beside_a_chunk(dev, seqs):
     rows[50] = 600
     parts, kernel, n = shared_call(dev, 128, 8, 1, lens, rows, held=sorted({0, 7, 20, 50, 77, seqs - 1}))
     assert np.all(kernel[n == 1] == 0) and np.all(kernel[n > 1] == 1)
+
+
+@pytest.mark.parametrize("D,H,KV,rows", [
+    (128, 8, 1, [3, 300, 2, 4]), (64, 8, 1, [4, 300, 1]), (64, 16, 1, [3, 300, 3]), (128, 16, 1, [3, 300, 4, 2]),
+    (256, 8, 1, [3, 300, 3]), (256, 4, 1, [4, 500, 1]), (128, 20, 1, [1, 300, 1]), (256, 20, 1, [1, 300, 1]),
+    (64, 40, 1, [1, 300, 1]), (128, 40, 1, [1, 300, 1]), (64, 64, 1, [1, 200, 1]),
+])
+def test_drafts_and_wide_groups_beside_a_chunk(dev, D, H, KV, rows):
+    """What the kernel of few rows holds goes to it: drafts, and many heads a kv head."""
+    lens = [9000 if n < 20 else 700 for n in rows]
+    parts, kernel, n = shared_call(dev, D, H, KV, lens, rows)
+    assert np.all(kernel[n < 20] == 0) and np.all(parts[n < 20] > 1) and np.all(kernel[n >= 20] == 1)
+
+
+def test_drafts_of_many_sequences_beside_a_chunk(dev):
+    rng = np.random.default_rng(4)
+    lens, rows = [int(n) for n in rng.integers(4, 900, 90)], [int(n) for n in rng.integers(1, 5, 90)]
+    lens[7], lens[50], rows[50] = 9000, 800, 600
+    parts, kernel, n = shared_call(dev, 128, 8, 1, lens, rows, held=[0, 7, 20, 50, 89])
+    assert np.all(kernel[n < 20] == 0) and np.all(kernel[n >= 20] == 1)

@@ -1079,7 +1079,18 @@ struct GqaPlans {
   bool both;
 };
 
-constexpr int kFewRows = 16;
+// Rows of the sequences that go to the kernel of few rows: one tile of it, or two
+// where a kv head's heads need them, or the mean rows of the others beside one
+// chunk.  8 sequences and a chunk of 512, in us: 3 rows of 8 heads at 131,072
+// tokens in the kernel of many rows (16 rows here) 1,494, in one tile of 32 515
+// (single rows 505 in both); of 16 heads 1,516, in two tiles 434, but single rows
+// 330 in one and 401 in two; at 256 channels, 65,536 tokens, 3 rows of 8 heads
+// 1,193 and 700, single rows 582 and 722.
+static int few_rows(int64_t tokens, int64_t seqs, int64_t max_rows, int group, int dim) {
+  const int one = dim == 256 ? 16 : 32;
+  const int64_t others = group * std::max<int64_t>((tokens - max_rows + seqs - 2) / std::max<int64_t>(seqs - 1, 1), 1);
+  return others > one && others <= 2 * one ? 2 * one : group <= one ? one : group <= 2 * one ? 2 * one : 0;
+}
 
 static GqaPlans dense_plans(int64_t tokens, int64_t seqs, int64_t max_rows, int group, int kv_heads, int dim,
                             int64_t max_len, int64_t window) {
@@ -1090,7 +1101,7 @@ static GqaPlans dense_plans(int64_t tokens, int64_t seqs, int64_t max_rows, int 
   };
   GqaPlans p{};
   p.all = gqa_plan(seqs, max_rows * group, tokens * group, kv_heads, dim, false, pages);
-  p.few_rows = group <= kFewRows ? kFewRows : 0;
+  p.few_rows = few_rows(tokens, seqs, max_rows, group, dim);
   // some sequence may have as few rows, of those that the call has in all
   const bool some = p.few_rows && tokens <= (seqs - 1) * max_rows + p.few_rows / group;
   p.both = p.all.row_tiles == 8 && some && pages(p.few_rows) >= 128 * p.all.splits;
