@@ -1132,15 +1132,17 @@ def _heads3(t: torch.Tensor, what: str) -> tuple:
     return T, H, D, t.data_ptr(), s0 if T > 1 else H * D, s1 if H > 1 else D
 
 
-def _bytes2(t: torch.Tensor, what: str) -> tuple:
-    """(address, row stride, rows) of uint8 [rows, bytes]."""
+def _bytes2(t: torch.Tensor, what: str, least: int) -> tuple:
+    """(address, row stride, rows) of uint8 [rows, bytes]; rows of fewer than
+    ``least`` bytes are as far apart as they are wide, which the library refuses:
+    part of a wider buffer is not written or read beside."""
     if t.dtype is not torch.uint8 or t.dim() != 2:
         _refuse(f"{what} uint8 [pages, bytes]")
     n, w = t.shape
     s0, s1 = t.stride()
     if s1 != 1:
         _refuse(f"{what} uint8 [pages, bytes] with unit byte stride")
-    return t.data_ptr(), s0 if n > 1 else w, n
+    return t.data_ptr(), s0 if n > 1 and w >= least else w, n
 
 
 def _table(t: torch.Tensor, rows: int) -> tuple:
@@ -1232,10 +1234,10 @@ def _append_args(k, v, positions, qsl, max_query_len, block_table, cache, summar
         _refuse("v must be [T, H_kv, D] like k")
     pos, seqs = _vector(positions, torch.int64, T, "positions"), _vector(qsl, torch.int32, 1, "qsl")
     B = qsl.numel() - 1
-    c, c0, pages = _bytes2(cache, "cache")
+    c, c0, pages = _bytes2(cache, "cache", KV * (128 * D + 8))
     s = s0 = 0
     if summary is not None:
-        s, s0, records = _bytes2(summary, "summary")
+        s, s0, records = _bytes2(summary, "summary", KV * (D + 4))
         if records < pages:
             _refuse("summary needs a record for each page")
     return ((kp, k0, k1, vp, v0, v1, T, KV, D),
@@ -1283,8 +1285,8 @@ def _gqa_attn_args(q, cache, kv_heads, block_table, seqs, positions, out, lse, s
             _refuse("lse fp32 [T, H]")
         l, l0 = lse.data_ptr(), lse.stride(0)
     s = None if sinks is None else _vector(sinks, torch.float32, H, "sinks")
-    return (T, H, D, (qp, q0, q1, T, H, kv_heads, D, *_bytes2(cache, "cache"), *_table(block_table, seqs),
-                      _vector(positions, torch.int64, T, "positions")), s, (op, o0, o1, l, l0))
+    return (T, H, D, (qp, q0, q1, T, H, kv_heads, D, *_bytes2(cache, "cache", kv_heads * (128 * D + 8)),
+                      *_table(block_table, seqs), _vector(positions, torch.int64, T, "positions")), s, (op, o0, o1, l, l0))
 
 
 def _gqa_workspace(workspace, need: int, like: torch.Tensor) -> tuple:
@@ -1342,8 +1344,9 @@ def gqa_block_select(q: torch.Tensor, summary: torch.Tensor, kv_heads: int, bloc
     T, H, D, qp, q0, q1 = _heads3(q, "q")
     if kv_heads <= 0 or H % kv_heads:
         _refuse("heads must be a multiple of kv_heads")
-    _gqa_call(dev, "ekv_gqa_block_select", qp, q0, q1, T, H, kv_heads, D, *_bytes2(summary, "summary"),
-              *_table(block_table, 0), _vector(positions, torch.int64, T, "positions"),
+    _gqa_call(dev, "ekv_gqa_block_select", qp, q0, q1, T, H, kv_heads, D,
+              *_bytes2(summary, "summary", kv_heads * (D + 4)), *_table(block_table, 0),
+              _vector(positions, torch.int64, T, "positions"),
               _vector(req_ids, torch.int32, T, "req_ids"), block_table.shape[0], max_len, keep_first, keep_last,
               *_block_lists(blocks, T, kv_heads))
 
