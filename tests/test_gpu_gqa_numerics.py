@@ -164,3 +164,26 @@ def test_small_values_beside_large_ones(dev, D, rows, H, first):
     out, lse = attend(layer, q, pos, np.array([0, rows], np.int32), rows, n, 1.0)
     check_weights(layer, q, out, lse, 1.0, [(t, 0) for t in sorted({0, rows // 2, rows - 1})], None,
                   lambda t, h: np.arange(pos[t] + 1))
+
+
+@pytest.mark.parametrize("D,rows,H", [(64, 1, 4), (128, 3, 16), (256, 1, 2), (64, 130, 2), (256, 130, 1)])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_scores_far_from_zero(dev, D, rows, H, sign):
+    """Scores of +-2^119, equal in all tokens (one product of powers of two): equal
+    weights, so that only the weights' and the result's roundings are left."""
+    rng = np.random.default_rng(D)
+    n = 64 * 20 + 9
+    layer = Layer(dev, rng, [n], 1, D, summary=False)
+    k = np.zeros((n, 1, D), np.float32)
+    k[..., 3] = sign * 2.0 ** 60
+    refill(layer, k, opposed(rng, n, 1, D))
+    q = np.zeros((rows, H, D), np.float32)
+    q[..., 3] = 2.0 ** 59
+    pos = np.arange(n - rows, n, dtype=np.int64)
+    out, lse = attend(layer, q, pos, np.array([0, rows], np.int32), rows, 20_000, 1.0)
+    _, vals = gqa.tokens(layer.cache, layer.bt[0], 1, D, 0)
+    for t in {0, rows // 2, rows - 1}:
+        v = vals[:pos[t] + 1]
+        tol = (2.0 ** -11 + (len(v) / 16 + 64) * 2.0 ** -24) * np.abs(v).mean(0) + 2.0 ** -8 * np.abs(v.mean(0))
+        assert np.all(np.abs(out[t] - v.mean(0)) <= tol)
+        assert np.all(np.abs(lse[t] / (sign * 2.0 ** 119) - 1) <= 2.0 ** -21)

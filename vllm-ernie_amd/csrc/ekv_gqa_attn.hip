@@ -15,7 +15,7 @@ namespace ekv {
 
 constexpr float kLog2e = 0x1.715476p+0f;
 constexpr float kLn2 = 0x1.62e430p-1f;
-constexpr float kNone = -1e30f;   // reference of a row that has seen no token
+constexpr float kNone = -0x1.fffffep127f;  // reference of a row that has seen no token: no score is below it
 // Weights are rounded to fp16 (11 bits, up to 65,504) for the product with V;
 // as bf16 their rounding was the largest error of a result (1.4 times that of
 // 32-bit weights, for 2% less time at 4,096 rows).  A reference lies 2^kLift
