@@ -187,3 +187,24 @@ def test_scores_far_from_zero(dev, D, rows, H, sign):
         tol = (2.0 ** -11 + (len(v) / 16 + 64) * 2.0 ** -24) * np.abs(v).mean(0) + 2.0 ** -8 * np.abs(v.mean(0))
         assert np.all(np.abs(out[t] - v.mean(0)) <= tol)
         assert np.all(np.abs(lse[t] / (sign * 2.0 ** 119) - 1) <= 2.0 ** -21)
+
+
+@pytest.mark.parametrize("D,H,KV", [(64, 4, 1), (128, 8, 2), (256, 2, 1)])
+def test_selection_by_the_largest_keys(dev, D, H, KV):
+    """Keys near the largest bf16 value: their scores, past 2^128, are still told apart."""
+    from ernie_kv import ops
+
+    rng = np.random.default_rng(D)
+    n = 64 * 40
+    layer = Layer(dev, rng, [n], KV, D)
+    k = rng.standard_normal((n, KV, D)) + 2 * rng.standard_normal((40, KV, D)).repeat(64, 0)
+    k *= 2.0 ** rng.integers(119, 124, (40, 1, 1)).repeat(64, 0)
+    k = bf16_round(np.clip(k, -3.3e38, 3.3e38).astype(np.float32))
+    gqa.append(k, k, np.arange(n), [0, n], layer.bt, layer.cache, layer.summary)
+    q = randn_bf16(rng, (5, H, D))
+    pos = np.array([n - 1, n - 70, 1000, 700, 64], np.int64)
+    ids = torch.empty((5, KV, 7), dtype=torch.int32, device=dev)
+    ops.gqa_block_select(bf16_tensor(q, dev), to_dev(layer.summary, dev), KV, layer.d_bt, to_dev(pos, dev),
+                         torch.zeros(5, dtype=torch.int32, device=dev), n, ids)
+    for t in range(5):
+        assert np.array_equal(ids[t].cpu().numpy(), gqa.select(q[t], layer.summary, KV, layer.bt[0], int(pos[t]), 7, 1, 2))

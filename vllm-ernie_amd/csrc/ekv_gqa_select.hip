@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(64 * WAVES) gqa_block_select_kernel(GqaSelectA
     if (pg >= a.num_pages || base + 64 * c + lane >= nb) pg = -1;
     live[buf] = pg >= 0;
     scale[buf] = 0.0f;
-    if (pg >= 0) scale[buf] = reinterpret_cast<const float*>(a.summary + pg * a.summary_stride + a.kv_heads * D)[h];
+    // 2^-24 of it, which leaves the order: products of up to 2^22 with scales of up to 2^122 stay finite
+    if (pg >= 0) scale[buf] = 0x1p-24f * reinterpret_cast<const float*>(a.summary + pg * a.summary_stride + a.kv_heads * D)[h];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int64_t p = __shfl(pg, 16 * u + m, 64);
