@@ -1048,13 +1048,17 @@ static GqaPlan gqa_plan(int64_t seqs, int64_t rows, int64_t all_rows, int kv_hea
   }
   // One round of the chip (32 rows of 64 listed pages, 8 kv heads, in parts:
   // 52 us in 768 workgroups, 56 in 2,048).
-  // Pages of a part.  Of many rows: shorter parts where units are fewer than CUs
-  // (4 sequences of 4,096 tokens, 16 rows, 8 kv heads of 128: 37 us at 16, 31 at
-  // 8), longer ones where each CU has one already (32 of 1,000: 50 us in two
-  // parts of 8, 35 in one), the shortest where most CUs have none (5 of 931 tokens,
-  // 8 rows of 12 heads a kv head of 256: 31 us at 8, 22 at 4; 224 units of 12
-  // pages: 47 and 51; the 4 of 4,096 again: 31 and 33).
-  const int64_t least = p.row_tiles < 8 || (p.units < 64 && pages >= 12 && pages <= 48) ? 4 : p.units < 256 ? 8 : 32;
+  // Pages of a part.  Of many rows: 8 where units are fewer than CUs (4 sequences
+  // of 4,096 tokens, 16 rows, 8 kv heads of 128: 37 us at 16, 31 at 8), longer
+  // ones where each CU has one already (32 of 1,000: 50 us in two parts of 8, 35
+  // in one), and 4 while such parts leave each a CU of its own.  At 4 and at 8, in
+  // us: 56 units of 128 channels, 16 pages 25 and 29, 20 pages 28 and 28, 40
+  // pages 44 and 37; 32 units, 32 pages 26 and 29, 64 pages 31 and 29; 8 units,
+  // 128 pages 25 and 29, 256 pages 33 and 30; 16 units of 256 channels, 64 pages
+  // 32 and 38, 80 pages 50 and 39; 1 unit of 64, 16 to 80 pages 14 to 16 and 18
+  // to 19.  Up to 8 pages stay one part, without a join (56 units of 8: 22 and
+  // 20; 8 units: 18 and 20).
+  const int64_t least = p.row_tiles < 8 || (pages > 8 && p.units * ((pages + 3) / 4) <= 256) ? 4 : p.units < 256 ? 8 : 32;
   int64_t splits = std::min<int64_t>({(round + (whole_rounds ? 0 : p.units - 1)) / std::max<int64_t>(p.units, 1),
                                       (pages + least - 1) / least, kMaxSplits});
   splits = std::max<int64_t>(splits, 1);
