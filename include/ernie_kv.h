@@ -780,6 +780,7 @@ int64_t ekv_gqa_attention_workspace_size(int32_t num_tokens, int32_t num_seqs, i
  * tokens j <= positions[t] and, with window > 0, j > positions[t] - window:
  *   out [T, heads, dim] bf16 = sum_j e^{s_j} v_j / (sum_j e^{s_j} + e^{sink}),
  *   s_j = scale q . k_j; lse [T, heads] fp32 = log sum_j e^{s_j} (may be NULL).
+ * Sums are fp32; for the product with v the weights are rounded to 11 bits.
  * scale > 0, finite; sinks [heads] fp32 may be NULL.  A row that sees no token (a negative
  * position) gets zeros and -inf; rows of no sequence are left as they were.
  * max_query_len and max_len bound the rows and the tokens of a sequence (heads of

@@ -177,7 +177,7 @@ __device__ __forceinline__ f16x8 fp8x8_to_f16(uint32_t lo, uint32_t hi, float s)
 // 2^-15 to 2^7: most pages' scales are within that of the first one's.  A page
 // whose scale is not moves the unit, and the sums with it; `top` is the largest
 // scale so far, 2^64 below which no unit goes, as the sums would overflow (values
-// 2^-75 of the largest ones' are taken as zeros there).
+// of pages whose scale is below 2^-75 of that lose bits).
 struct ValueUnit {
   int at = -1000, top = -1000;
 };
@@ -755,16 +755,16 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
 // Many rows a kv head: one workgroup per (128 rows, kv head, range of pages).
 // Its waves (4 of 32 rows; 8 of 16 at 256 channels, whose sums of 32 would leave
 // one wave a SIMD: 1,490 -> 1,100 us at 2,048 rows) share every page: each brings
-// its part of it, converted to bf16 once, into LDS in the order of the operands
-// (1 KB reads of 64 consecutive 16-byte pieces, no bank conflicts), while the
+// its part of it, converted once (K to bf16, as q is, V to fp16, as the weights
+// are), into LDS in the order of the operands (1 KB reads of 64 consecutive 16-byte pieces, no bank conflicts), while the
 // page before is multiplied.
 //
 // Bound by the matrix cores and the weights' exponentials, which two waves a
-// SIMD overlap in part (4,096 rows of 32 heads of 128 at 32,768 tokens: 1,776 to
-// 1,860 us, 1,110 to 1,160 TFLOP/s, matrix cores busy 46% of the cycles; a
+// SIMD overlap in part (4,096 rows of 32 heads of 128 at 32,768 tokens: 1,784 to
+// 1,844 us, 1,118 to 1,156 TFLOP/s, matrix cores busy 46% of the cycles; a
 // product of 8,192^3 reaches 1,128 on the same card, of 16,384^3 1,350).  At 64
-// channels the exponentials are half of the work (2,048 rows at 16,384: 780
-// TFLOP/s), at 256 there are more conversions a product (940).
+// channels the exponentials are half of the work (2,048 rows of 64 heads at
+// 16,384: 810 TFLOP/s), at 256 there are more conversions a product (930).
 // ---------------------------------------------------------------------------
 template <int D>
 struct PrefillShape {
@@ -985,7 +985,7 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(GqaAttnArgs a, int slo
 // Host side
 // ---------------------------------------------------------------------------
 struct GqaPlan {
-  int row_tiles;  // 16-row tiles of a workgroup: 1, 2, 4 in every wave, or 8 over its four waves
+  int row_tiles;  // 16-row tiles of a workgroup: 1, 2, 4 in every wave, or 8 over its four (256 channels: eight) waves
   int tiles, splits, split_pages, budget;
   int64_t units, slots;  // slots: workgroups
   bool join, wide, by_rows;
