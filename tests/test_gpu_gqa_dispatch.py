@@ -148,3 +148,43 @@ def test_drafts_of_many_sequences_beside_a_chunk(dev):
     lens[7], lens[50], rows[50] = 9000, 800, 600
     parts, kernel, n = shared_call(dev, 128, 8, 1, lens, rows, held=[0, 7, 20, 50, 89])
     assert np.all(kernel[n < 20] == 0) and np.all(kernel[n >= 20] == 1)
+
+
+@pytest.mark.parametrize("D,window", [(64, 0), (128, 100_000), (256, 0)])
+def test_captured_mixed_call(dev, D, window):
+    """Single rows, a draft and chunks in one captured call, both kernels and
+    their joins: each replay gives the eager bytes, also on another stream and
+    after other calls' use of the workspace."""
+    from ernie_kv import ops
+
+    rng = np.random.default_rng(D)
+    H, KV, lens, rows = 8, 1, [9000, 500, 2000, 700], [1, 300, 2, 200]
+    layer = Layer(dev, rng, lens, KV, D, summary=False)
+    q, pos, seq, qsl = batch(rng, lens, rows, H, D)
+    tq, tpos, tqsl = bf16_tensor(q, dev), to_dev(pos, dev), to_dev(qsl, dev)
+    out, lse = torch.empty_like(tq), torch.empty(tq.shape[:2], device=dev)
+    ws = torch.empty(size(q, qsl, 300, 1 << 20, KV, window), dtype=torch.uint8, device=dev)
+
+    def step(workspace):
+        ops.gqa_attention(tq, layer.d_cache, KV, layer.d_bt, tpos, tqsl, 300, 1 << 20, D ** -0.5, out, lse, window=window,
+                          workspace=workspace)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(ws)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(ws)
+    for rep in range(4):
+        tq.copy_(bf16_tensor(randn_bf16(rng, q.shape), dev))
+        step(None)
+        want = out.clone(), lse.clone()
+        out.fill_(7), lse.fill_(7), ws.fill_((0, 2, 255, 1)[rep])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side if rep % 2 else torch.cuda.current_stream()):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1]), f"replay {rep}"

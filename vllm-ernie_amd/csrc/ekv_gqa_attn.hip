@@ -258,8 +258,8 @@ struct RowRange {
 // Scores x (token 16 j + 4 g + i of the page, row n) -> weights around the
 // rows' references m, as the B operand of the product with V, and their sums.
 // kscale > 0 takes a raw score to log2 units.  A reference is a maximum that the
-// row has had, less kLift, and moves only where the page's weights around it grow past
-// kMoveAt.  kBySum sees that in their sums, which costs no maximum but the raw
+// row has had, less kLift, and moves only where the page's weights around it grow
+// past kMoveAt.  kBySum sees that in their sums, which costs no maximum but the raw
 // scores' registers (many rows, where the products bound the kernel: 3% less time
 // at 4,096 rows); else in the largest score.  Masks are selects without branches.
 template <bool kBySum, int NT, int DT>
@@ -756,8 +756,8 @@ __global__ void __launch_bounds__(64 * W, (kDecodeWaves<D, NT>)) gqa_decode_kern
 // Its waves (4 of 32 rows; 8 of 16 at 256 channels, whose sums of 32 would leave
 // one wave a SIMD: 1,490 -> 1,100 us at 2,048 rows) share every page: each brings
 // its part of it, converted once (K to bf16, as q is, V to fp16, as the weights
-// are), into LDS in the order of the operands (1 KB reads of 64 consecutive 16-byte pieces, no bank conflicts), while the
-// page before is multiplied.
+// are), into LDS in the order of the operands (1 KB reads of 64 consecutive
+// 16-byte pieces, no bank conflicts), while the page before is multiplied.
 //
 // Bound by the matrix cores and the weights' exponentials, which two waves a
 // SIMD overlap in part (4,096 rows of 32 heads of 128 at 32,768 tokens: 1,784 to
