@@ -27,7 +27,8 @@ def check_weights(layer, q, out, lse, scale, rows, sinks, seen):
     it; of one far below, half the smallest fp16 step, which is 2^-30 of the row's
     largest: 2^-25 where that is 2^5 or more), a score's fp32 sum (D + 8 steps of
     2^-24 of sum |q k|) and the sum of n weights ((n / 16 + 64) 2^-24), each of
-    which moves the weights by as much, and the result rounded to bf16 once.  Rounding the weights to bf16 would be off by up to 2^-8 of sum |w v|."""
+    which moves the weights by as much, and the result rounded to bf16 once.
+    Weights rounded to bf16 would be off by up to 2^-8 of sum |w v|."""
     H, D, KV = q.shape[1], q.shape[2], layer.KV
     G, worst = H // KV, 0.0
     for t, b in rows:
